@@ -386,6 +386,69 @@ int nerf_mlp_wgrad_config(int n_feat, int k_feat, int* nw, int* tn, int* tk, int
  * the launch (0 = segment absent). */
 int nerf_mlp_wgrad8_config(int n_feat0, int n_feat1, int k_feat0, int k_feat1, int* tn, int* tk, int* gs);
 
+/* ---- (f) gradient norm, clipping, optimizer step over a list of tensors ------------------- */
+
+/* What lies between a backward pass and the next forward pass.  The lists are HOST arrays of n_tensors device pointers,
+ * element counts and element types (NERF_F32 / NERF_BF16 / NERF_F16, mixed as one likes); the tensors are dense, their
+ * element order does not matter, and they may start at any multiple of their element size.  The arrays are read before
+ * the call returns.  `workspace`: nerf_grad_workspace_bytes(n_tensors) bytes of device scratch, 8-byte aligned, whose
+ * contents mean nothing between calls; calls that may overlap on the device each need their own.  Sums and norms are held
+ * in 64 bits and added in a fixed order: the same bits on every call, and no overflow or underflow of the squares.
+ *                              reference: torch.optim.AdamW (model.py:177-181); it has no clipping */
+#define NERF_F32 0
+#define NERF_BF16 1
+#define NERF_F16 2
+
+#define NERF_NORM_NONE 0
+#define NERF_NORM_L1 1
+#define NERF_NORM_L2 2
+#define NERF_NORM_MAX 3
+
+/* Bytes of workspace that the calls below need for a list of n_tensors (NERF_ERR_ARG if negative). */
+int64_t nerf_grad_workspace_bytes(int n_tensors);
+
+/* norm[1] (fp32) = the norm of all entries of all tensors together: sum |g|, sqrt(sum g^2) or max |g|.  A NaN entry
+ * gives NaN, an infinite one inf; an empty list 0. */
+int nerf_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtype, int n_tensors, int norm_kind,
+                   void* workspace, int64_t workspace_bytes, float* norm, void* stream);
+
+/* g *= min(1, max_norm / (norm + 1e-6)), in place, for every entry of every tensor; norm[1] receives the norm before.
+ * Products are taken in fp32 and rounded once to the tensor's type.  A NaN norm makes every entry NaN; with an infinite
+ * one finite entries become 0 and infinite ones NaN.  The tensors must not share memory (NERF_ERR_ARG). */
+int nerf_clip_grad_norm(void* const* grads, const int64_t* numel, const int32_t* dtype, int n_tensors, int norm_kind,
+                        double max_norm, void* workspace, int64_t workspace_bytes, float* norm, void* stream);
+
+/* One AdamW step (decoupled weight decay) over a list of parameters, with the gradients clipped as they are read:
+ *   g' = min(1, max_norm / (norm + 1e-6)) g      (norm_kind = NERF_NORM_NONE: g' = g, max_norm and norm unused)
+ *   m = beta1 m + (1 - beta1) g',   v = beta2 v + (1 - beta2) g'^2,   step = step + 1
+ *   w -= lr (m / (1 - beta1^step) / (sqrt(v / (1 - beta2^step)) + eps) + weight_decay w)
+ * grads are not written.  exp_avg, exp_avg_sq (fp32) and step (one fp32 per parameter, on the device) are read and
+ * written; so are `master` weights (fp32, for 16-bit parameters; unused for NERF_F32, the array may be NULL if there are
+ * none).  A 16-bit parameter is w rounded to nearest; where it is no longer that (it was written from outside) the
+ * master restarts from the parameter.  `dtype` is that of the parameter and of its gradient.  skip_nonfinite != 0 (with a
+ * norm): where the norm is infinite or NaN nothing but `norm` is written.  groups[k] holds the settings of the next
+ * `count` parameters of the list; lr_device (nullable) is an fp32 learning rate on the device, read in place of `lr`.
+ * norm[1] (nullable) receives the norm before clipping, over all groups.  Parameters must not share memory. */
+typedef struct nerf_adamw_tensors {
+    int n_tensors;
+    void* const* param;
+    const void* const* grad;
+    float* const* exp_avg;
+    float* const* exp_avg_sq;
+    float* const* master;
+    float* const* step;
+    const int64_t* numel;
+    const int32_t* dtype;
+} nerf_adamw_tensors;
+typedef struct nerf_adamw_group {
+    int count;
+    const float* lr_device;
+    double lr, beta1, beta2, eps, weight_decay;
+} nerf_adamw_group;
+int nerf_adamw_step(const nerf_adamw_tensors* tensors, const nerf_adamw_group* groups, int n_groups, int norm_kind,
+                    double max_norm, int skip_nonfinite, void* workspace, int64_t workspace_bytes, float* norm,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

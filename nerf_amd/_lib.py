@@ -6,7 +6,7 @@ call raises.
 """
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
 
@@ -21,6 +21,16 @@ class NerfActivation(Structure):
 
 class MlpDims(Structure):
     _fields_ = [('enc_dim', c_int), ('view_dim', c_int), ('hidden', c_int), ('width', c_int), ('sar', c_int)]
+
+
+class AdamwTensors(Structure):
+    _fields_ = [('n_tensors', c_int), ('param', c_void_p), ('grad', c_void_p), ('exp_avg', c_void_p),
+                ('exp_avg_sq', c_void_p), ('master', c_void_p), ('step', c_void_p), ('numel', c_void_p), ('dtype', c_void_p)]
+
+
+class AdamwGroup(Structure):
+    _fields_ = [('count', c_int), ('lr_device', c_void_p), ('lr', c_double), ('beta1', c_double), ('beta2', c_double),
+                ('eps', c_double), ('weight_decay', c_double)]
 
 
 _P = c_void_p
@@ -58,6 +68,11 @@ _SIGS = {
     'nerf_layernorm_fwd': (c_int, [_P, _P, _P, c_int64, c_int, c_float, _P, _P, _P, _P]),
     'nerf_layernorm_bwd': (c_int, [_P, _P, _P, _P, _P, c_int64, c_int, _P, _P, _P, _P]),
     'nerf_sar_pulse_loss': (c_int, [_P, _P, _P, c_int, c_int, c_int, c_float, _P, _P, _P, _P]),
+    'nerf_grad_workspace_bytes': (c_int64, [c_int]),
+    'nerf_grad_norm': (c_int, [_P, _P, _P, c_int, c_int, _P, c_int64, _P, _P]),
+    'nerf_clip_grad_norm': (c_int, [_P, _P, _P, c_int, c_int, c_double, _P, c_int64, _P, _P]),
+    'nerf_adamw_step': (c_int, [POINTER(AdamwTensors), POINTER(AdamwGroup), c_int, c_int, c_double, c_int, _P, c_int64,
+                                _P, _P]),
 }
 
 _lib = None

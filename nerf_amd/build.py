@@ -27,6 +27,7 @@ UNITS = {
     'composite.o': ('composite.hip', ['-ffp-contract=off']),
     'sar_pulse.o': ('sar_pulse.hip', []),
     'gemm_f32.o': ('gemm_f32.hip', []),
+    'optimizer.o': ('optimizer.hip', ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']),
     # VGPR-form matrix-core instructions where an accumulator tile lives in the vector registers: the outputs of the
     # larger launches exceed the 256 accumulation registers, and the default form copies such tiles in and out
     # of them around every product (layer 4's launch: 1.10 -> 0.86 ms)

@@ -4,6 +4,8 @@ autograd.  All tensors are flattened to `[N, ...]` rays here; shape handling for
 reference-compatible surface lives in `nerf_amd.utils`.
 """
 import ctypes
+import math
+from array import array
 
 import torch
 
@@ -259,3 +261,108 @@ def sar_pulse_loss(pulse, mfilt, target, coarse_weight, need_grad=True, need_pro
                                     stream()))
     loss = coarse_weight * mse[:-1].sum() + mse[-1]
     return loss, mse, profile, g
+
+
+# ---- gradient norm, clipping, optimizer step over a list of tensors (csrc/optimizer.hip) ----------------------------
+
+LIST_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+NORM_KINDS = {1.0: 1, 2.0: 2, math.inf: 3}
+
+
+def norm_kind(norm_type):
+    """The C ABI's code of a norm's order: 1, 2 or inf (the largest entry)."""
+    kind = NORM_KINDS.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f'norm_type must be 1, 2 or inf, got {norm_type!r}')
+    return kind
+
+
+def check_max_norm(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f'max_norm must not be negative or NaN, got {max_norm!r}')
+    return max_norm
+
+
+def list_device(tensors):
+    """The index of the one HIP device that holds every tensor of a list."""
+    devices = {t.get_device() for t in tensors}
+    if len(devices) > 1:
+        raise RuntimeError('nerf_amd kernels need the tensors of a list on one HIP device')
+    dev = devices.pop()
+    if dev < 0:
+        raise RuntimeError('nerf_amd kernels need tensors on a HIP device; got a CPU tensor')
+    return dev
+
+
+def list_dtypes(tensors):
+    try:
+        return array('i', [LIST_DTYPES[t.dtype] for t in tensors])
+    except KeyError as e:
+        raise RuntimeError(f'expected float32, bfloat16 or float16 tensors, got {e.args[0]}') from None
+
+
+def is_dense(t):
+    """Whether the entries of `t` fill a stretch of memory without gaps or overlaps, in whatever order."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _addr(a):
+    return a.buffer_info()[0]
+
+
+def ptr_array(tensors):
+    return array('Q', [t.data_ptr() for t in tensors])
+
+
+def _list_call(entry, tensors, *args):
+    """entry(pointers, numels, dtypes, n, *args, workspace, bytes, norm, stream) on the device that holds the list
+    -> the norm, a 0-d fp32 tensor."""
+    n = len(tensors)
+    dev = list_device(tensors) if n else torch.cuda.current_device()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _list_call(entry, tensors, *args)
+    ptrs, dtypes = ptr_array(tensors), list_dtypes(tensors)
+    numels = array('q', [t.numel() for t in tensors])
+    nbytes = lib().nerf_grad_workspace_bytes(n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device='cuda')
+    norm = torch.empty((), dtype=torch.float32, device='cuda')
+    check(entry(_addr(ptrs), _addr(numels), _addr(dtypes), n, *args, ws.data_ptr(), nbytes, norm.data_ptr(), stream()))
+    return norm
+
+
+def _as_list(tensors):
+    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+
+
+def grad_norm(tensors, norm_type=2.0):
+    """The norm of all entries of a list of tensors (or of one tensor) together: `norm_type` 2, 1 or inf -> a 0-d fp32
+    tensor on their device (no host synchronisation).  fp32, bf16 and fp16 tensors in one list as one likes; sums are held
+    in 64 bits and added in a fixed order.  A NaN entry gives NaN; an empty list gives 0.  No gradient flows through it."""
+    kind = norm_kind(norm_type)
+    tensors = _as_list(tensors)
+    if not all(t.is_contiguous() for t in tensors):     # any dense order will do; anything else is copied
+        tensors = [t if is_dense(t) else t.detach().contiguous() for t in tensors]
+    return _list_call(lib().nerf_grad_norm, tensors, kind)
+
+
+def clip_grad_norm_(tensors, max_norm, norm_type=2.0):
+    """Scale a list of gradient tensors (or one) in place by min(1, max_norm / (norm + 1e-6)) -> the norm before, a 0-d
+    fp32 tensor (no host synchronisation).  Products are taken in fp32 and rounded once.  A norm that is not finite is
+    carried into the gradients as the product says: NaN makes every entry NaN, inf makes finite entries 0.  The tensors
+    must be dense (any order of dimensions) and must not share memory."""
+    kind, max_norm = norm_kind(norm_type), check_max_norm(max_norm)
+    tensors = _as_list(tensors)
+    if not all(t.is_contiguous() or is_dense(t) for t in tensors):
+        raise RuntimeError('clip_grad_norm_: expected dense tensors (no gaps, no broadcast dimensions)')
+    norm = _list_call(lib().nerf_clip_grad_norm, tensors, kind, max_norm)
+    torch.autograd.graph.increment_version(tensors)     # (the kernels write behind autograd's back)
+    return norm

@@ -1,0 +1,197 @@
+"""Gradient clipping and the AdamW step on the HIP kernels of csrc/optimizer.hip: what a training loop does between a
+backward pass and the next forward pass.
+
+`clip_grad_norm_` takes parameters and clips their gradients; `AdamW` is a `torch.optim.Optimizer` (learning-rate
+schedulers, parameter groups, `state_dict` as torch's own AdamW, model.py:177-181) whose step is two launches for all
+parameters together, takes the gradients' norm and clips them while it reads them, and can be captured into a HIP graph.
+The tensor-level entry points are `nerf_amd.ops.grad_norm` and `nerf_amd.ops.clip_grad_norm_`.
+"""
+import ctypes
+from array import array
+
+import torch
+
+from . import ops
+from ._lib import AdamwGroup, AdamwTensors, check, lib, stream
+
+_addr = ops._addr
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Clip the gradients of `parameters` (an iterable, or one tensor) by their norm taken together, in place -> the norm
+    before, a 0-d fp32 tensor.  Parameters without a gradient are passed over.  With `error_if_nonfinite` the norm is
+    read back (one stream synchronisation) and a norm that is not finite raises with the gradients as they were."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if error_if_nonfinite:
+        norm = ops.grad_norm(grads, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f'clip_grad_norm_: the gradients\' norm of order {norm_type} is not finite')
+    return ops.clip_grad_norm_(grads, max_norm, norm_type)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay; arguments as torch.optim.AdamW's, and
+
+    max_norm         the gradients are scaled by min(1, max_norm / (norm + 1e-6)) as they are read (`.grad` itself is not
+                     written); the norm is taken over all parameter groups together.  None: no clipping.
+    norm_type        2, 1 or inf.
+    skip_nonfinite   a step whose gradient norm is infinite or NaN leaves parameters, moments and step counters as they are.
+
+    `grad_norm` holds the norm of the last step (a 0-d fp32 tensor on the device; None before the first, and without
+    max_norm or skip_nonfinite).  Parameters are fp32, bf16 or fp16, on one HIP device, their gradients of the same type.
+    The moments are fp32 whatever the parameters are, and a 16-bit parameter has an fp32 master weight in the state
+    ('master'), of which it is the rounding.  The step counters live on the device, so a captured step counts on with
+    every replay; the learning rate of a group may be an fp32 device tensor, which a replay reads afresh.  The state is
+    laid out by the first step, which therefore cannot be a captured one."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, norm_type=2.0,
+                 skip_nonfinite=False):
+        if not torch.is_tensor(lr) and not lr >= 0.0:
+            raise ValueError(f'invalid learning rate: {lr}')
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f'invalid betas: {betas}')
+        if not eps >= 0.0:
+            raise ValueError(f'invalid eps: {eps}')
+        if not weight_decay >= 0.0:
+            raise ValueError(f'invalid weight_decay: {weight_decay}')
+        self.max_norm = None if max_norm is None else ops.check_max_norm(max_norm)
+        self._kind = ops.norm_kind(norm_type)
+        self.norm_type, self.skip_nonfinite = float(norm_type), bool(skip_nonfinite)
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, capturable=True))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for g in self.param_groups:
+            g['capturable'] = True
+
+    def load_state_dict(self, state_dict):
+        """A state dict of this class or of torch.optim.AdamW (without amsgrad / maximize)."""
+        for g in state_dict['param_groups']:
+            if g.get('amsgrad') or g.get('maximize'):
+                raise ValueError('AdamW: amsgrad and maximize are not supported')
+        super().load_state_dict(state_dict)
+        # The base class gives floating-point state the parameter's type and may leave step counters on the host: the
+        # moments and masters are fp32 here, and the counters live beside them.
+        ids = [i for g in state_dict['param_groups'] for i in g['params']]
+        for i, p in zip(ids, [p for g in self.param_groups for p in g['params']]):
+            saved = state_dict['state'].get(i)
+            if not saved:
+                continue
+            st = {k: torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(saved[k])
+                  for k in ('exp_avg', 'exp_avg_sq', 'master') if k in saved}
+            st['step'] = torch.as_tensor(saved['step'], dtype=torch.float32).to(p.device, copy=True).reshape(())
+            self.state[p] = st
+        for g in self.param_groups:
+            for k in list(g):
+                if k not in self.defaults and k not in ('params', 'initial_lr', 'param_names'):
+                    del g[k]
+            g['capturable'] = True
+
+    def _init_state(self, params):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('AdamW: run one step ahead of a graph capture (it lays out the optimizer state; captured, '
+                               'every replay would clear it)')
+        steps = torch.zeros(len(params), dtype=torch.float32, device=params[0].device)
+        for i, p in enumerate(params):
+            st = self.state[p]
+            st['step'] = steps[i]
+            st['exp_avg'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+            st['exp_avg_sq'] = torch.zeros_like(st['exp_avg'])
+
+    def _check_state(self, p, st):
+        """State that came from outside has to be what the kernel reads: fp32, on the device, laid out as the parameter."""
+        for k in ('exp_avg', 'exp_avg_sq', 'master'):
+            t = st.get(k)
+            if t is not None and (t.dtype != torch.float32 or t.get_device() != p.get_device() or t.shape != p.shape
+                                  or not (t.stride() == p.stride() or t.is_contiguous() and p.is_contiguous())):
+                raise RuntimeError(f'AdamW: state {k!r} must be an fp32 tensor of the parameter\'s shape, order and device')
+        t = st['step']
+        if t.dtype != torch.float32 or t.get_device() != p.get_device() or t.numel() != 1:
+            raise RuntimeError('AdamW: state \'step\' must be one fp32 number on the parameter\'s device')
+
+    def _grad_of(self, p):
+        g = p.grad
+        if g.is_sparse or g.dtype != p.dtype or g.get_device() != p.get_device():
+            raise RuntimeError('AdamW: gradients must be dense tensors of their parameters\' type and device')
+        if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+            # another order of the same entries: laid out as the parameter is
+            g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
+        return g
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params, counts = [], []
+        for group in self.param_groups:
+            with_grad = [p for p in group['params'] if p.grad is not None]
+            counts.append(len(with_grad))
+            params += with_grad
+        clips = self.max_norm is not None or self.skip_nonfinite
+        if not params:
+            if clips:
+                p = next((p for g in self.param_groups for p in g['params']), None)
+                self.grad_norm = torch.zeros((), device=p.device if p is not None else None)
+            return loss
+        dev = ops.list_device(params)
+        if dev != torch.cuda.current_device():
+            with torch.cuda.device(dev):
+                self._step(params, counts, clips)
+        else:
+            self._step(params, counts, clips)
+        return loss
+
+    def _step(self, params, counts, clips):
+        dtypes = ops.list_dtypes(params)
+        for p in params:
+            if not (p.is_contiguous() or ops.is_dense(p)):
+                raise RuntimeError('AdamW: expected dense parameters')
+        grads = [self._grad_of(p) for p in params]
+        fresh = [p for p in params if 'exp_avg' not in self.state[p]]
+        if fresh:
+            self._init_state(fresh)
+        states = [self.state[p] for p in params]
+        half = any(dtypes)
+        if half:
+            for p, st in zip(params, states):
+                if p.dtype != torch.float32 and 'master' not in st:
+                    st['master'] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
+        for p, st in zip(params, states):
+            self._check_state(p, st)
+        n = len(params)
+        arrays = [ops.ptr_array(params), ops.ptr_array(grads), ops.ptr_array([s['exp_avg'] for s in states]),
+                  ops.ptr_array([s['exp_avg_sq'] for s in states]),
+                  array('Q', [s['master'].data_ptr() if 'master' in s else 0 for s in states]),
+                  ops.ptr_array([s['step'] for s in states]), array('q', [p.numel() for p in params]), dtypes]
+        table = AdamwTensors(n, *(_addr(a) for a in arrays))
+        groups = (AdamwGroup * len(counts))()
+        for c, count, g in zip(groups, counts, self.param_groups):
+            lr = g['lr']
+            c.count = count
+            if torch.is_tensor(lr):
+                if lr.numel() != 1:
+                    raise ValueError('AdamW: a tensor learning rate must have one element')
+                if lr.is_cuda:
+                    if lr.dtype != torch.float32 or lr.get_device() != params[0].get_device():
+                        raise ValueError('AdamW: a tensor learning rate must be fp32 on the parameters\' device')
+                    c.lr_device = lr.data_ptr()
+                else:
+                    c.lr = float(lr)
+            else:
+                c.lr = float(lr)
+            c.beta1, c.beta2 = g['betas']
+            c.eps, c.weight_decay = g['eps'], g['weight_decay']
+        nbytes = lib().nerf_grad_workspace_bytes(n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device='cuda')
+        norm = torch.empty((), dtype=torch.float32, device='cuda') if clips else None
+        max_norm = float('inf') if self.max_norm is None else self.max_norm
+        check(lib().nerf_adamw_step(ctypes.byref(table), groups, len(counts), self._kind if clips else 0, max_norm,
+                                    int(self.skip_nonfinite), ws.data_ptr(), nbytes, norm.data_ptr() if clips else None,
+                                    stream()))
+        if clips:
+            self.grad_norm = norm
+        torch.autograd.graph.increment_version(params)      # (the kernels write behind autograd's back)
