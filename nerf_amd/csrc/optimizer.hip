@@ -8,10 +8,10 @@
 //
 // All of it is bound by memory.  The tensors of a list reach a kernel by value, as a table in its arguments (no copy
 // to the device, nothing that a captured graph would have to keep alive); a list longer than a table goes out as
-// several launches.  Each tensor is cut into chunks, one workgroup per chunk.  The norm is one launch that leaves a
-// partial sum per chunk in the caller's workspace; every workgroup of the launch that needs the norm adds those up for
-// itself, in one fixed order, so that there are no atomics, no waiting between workgroups, no launch in between, and
-// the same bits on every call.
+// several launches.  Each tensor is cut into chunks, which the workgroups of a launch take in turn, so that all of them
+// together sweep through memory.  The norm is one launch that leaves a partial sum per workgroup in the caller's
+// workspace; every workgroup of the launch that needs the norm adds those up for itself, in one fixed order, so that
+// there are no atomics, no waiting between workgroups, no launch in between, and the same bits on every call.
 #include <stdlib.h>
 
 #include <algorithm>
@@ -22,28 +22,28 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kNormCap = 128;       // tensors per launch: the tables stay below 4 KB of kernel arguments
-constexpr int kScaleCap = 128;
-constexpr int kAdamCap = 64;
+constexpr int kNormCap = 112;       // tensors per launch: the tables stay below 4 KB of kernel arguments
+constexpr int kScaleCap = 176;
+constexpr int kAdamCap = 56;
 constexpr int kStepCap = 256;
-constexpr int kMaxPartials = 2048;  // chunks of one call: at most this many, and one more per tensor
+constexpr int kMaxGroups = 2048;    // workgroups of one launch: eight per compute unit
 constexpr int kMinChunk = 1024;
+constexpr int kMaxChunk = 16384;
 
 struct NormTable {
     const void* ptr[kNormCap];
     const float* step[kNormCap];    // null, or the tensor's step counter: copied to the workspace
     int64_t numel[kNormCap];
     int end[kNormCap];              // chunks of the tensors up to and including this one
-    int n, first_tensor, first_partial;
-    int64_t chunk;
+    int id[kNormCap];               // place in the caller's list
+    int n, first_partial, chunk;
 };
 
 struct ScaleTable {
     void* ptr[kScaleCap];
     int64_t numel[kScaleCap];
     int end[kScaleCap];
-    int n;
-    int64_t chunk;
+    int n, chunk;
 };
 
 struct AdamTable {
@@ -55,8 +55,8 @@ struct AdamTable {
     float* step[kAdamCap];
     int64_t numel[kAdamCap];
     int end[kAdamCap];
-    int n, first_tensor;
-    int64_t chunk;
+    int id[kAdamCap];
+    int n, chunk;
 };
 
 struct StepTable {
@@ -78,19 +78,42 @@ struct AdamArgs {
     double ln1, ln2;                // ln(beta)
 };
 
-// The table entry that a chunk belongs to.  The lanes of a wave compare 64 entries at a time: two loads deep, where a
-// bisection through the kernel's arguments would be six or seven.
-template <int CAP>
-__device__ __forceinline__ int find_tensor(const int (&end)[CAP], int n, int chunk) {
-    int idx = 0;
+// A stretch [lo, hi) of tensor t, as chunk b of a table.  The lanes of a wave compare 64 entries at a time: two loads
+// deep, where a bisection through the kernel's arguments would be six or seven.
+struct Chunk {
+    int t;
+    bool first;         // of its tensor
+    int64_t lo, hi;
+};
+
+template <typename Table, int CAP>
+__device__ __forceinline__ Chunk find_chunk(const Table& tab, const int (&end)[CAP], int b) {
+    int t = 0;
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int base = 0; base < CAP; base += 64) {
         const int i = base + lane;
-        idx += __popcll(__ballot(i < n && end[i < n ? i : 0] <= chunk));
+        t += __popcll(__ballot(i < tab.n && end[i < tab.n ? i : 0] <= b));
     }
-    return __builtin_amdgcn_readfirstlane(idx);
+    t = __builtin_amdgcn_readfirstlane(t);
+    const int first = t ? end[t - 1] : 0;
+    Chunk c;
+    c.t = t;
+    c.first = b == first;
+    c.lo = (int64_t)(b - first) * tab.chunk;
+    c.hi = c.lo + tab.chunk < tab.numel[t] ? c.lo + tab.chunk : tab.numel[t];
+    return c;
 }
+
+// Sixteen bytes per lane and access.  A tensor may start at any multiple of its element size, so the type promises no
+// more than that; the hardware takes such addresses in one access all the same.
+template <typename T, int N>
+struct Pack {
+    typedef T type __attribute__((ext_vector_type(N)));
+    typedef type loose __attribute__((aligned(sizeof(T))));
+    static __device__ __forceinline__ type load(const T* p) { return *(const loose*)p; }
+    static __device__ __forceinline__ void store(T* p, type x) { *(loose*)p = x; }
+};
 
 // ---- sums in a fixed order --------------------------------------------------------------------------------------
 // Sums are held in 64 bits: the square of a 32-bit value is exact there, and neither overflows nor underflows, so the
@@ -134,25 +157,41 @@ __device__ __forceinline__ float coefficient(double norm, double max_norm) {
     return d <= max_norm ? 1.f : (float)(max_norm / d);       // (a NaN norm gives NaN)
 }
 
+template <int KIND>
+__device__ __forceinline__ double take(double acc, float x) {
+    if (KIND == NERF_NORM_L2) return fma((double)x, (double)x, acc);
+    return join<KIND>(acc, (double)fabsf(x));
+}
+
 template <typename T, int KIND>
 __global__ __launch_bounds__(kThreads) void norm_partials(NormTable tab, double* partials, float* steps) {
-    const int b = blockIdx.x;
-    const int t = find_tensor(tab.end, tab.n, b);
-    const int first = t ? tab.end[t - 1] : 0;
-    const T* g = (const T*)tab.ptr[t];
-    const int64_t lo = (int64_t)(b - first) * tab.chunk;
-    const int64_t hi = lo + tab.chunk < tab.numel[t] ? lo + tab.chunk : tab.numel[t];
-    double acc = 0.0;
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
-        const float x = (float)g[i];
-        if (KIND == NERF_NORM_L2) acc = fma((double)x, (double)x, acc);
-        else acc = join<KIND>(acc, (double)fabsf(x));
+    constexpr int V = 16 / sizeof(T), kStep = kThreads * V, kDeep = 4;
+    using P = Pack<T, V>;
+    double acc[2] = {0.0, 0.0};
+    const int total = tab.end[tab.n - 1];
+    for (int b = blockIdx.x; b < total; b += gridDim.x) {
+        const Chunk c = find_chunk(tab, tab.end, b);
+        const T* g = (const T*)tab.ptr[c.t];
+        int64_t i = c.lo + threadIdx.x * V;
+        for (; i + (kDeep - 1) * kStep + V <= c.hi; i += kDeep * kStep) {
+            typename P::type x[kDeep];
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) x[k] = P::load(g + i + k * kStep);
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) acc[j & 1] = take<KIND>(acc[j & 1], (float)x[k][j]);
+        }
+        for (; i + V <= c.hi; i += kStep) {
+            const typename P::type x = P::load(g + i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j & 1] = take<KIND>(acc[j & 1], (float)x[j]);
+        }
+        for (; i < c.hi; ++i) acc[0] = take<KIND>(acc[0], (float)g[i]);     // the last lane's rest
+        if (c.first && threadIdx.x == 0 && tab.step[c.t]) steps[tab.id[c.t]] = *tab.step[c.t];
     }
-    acc = group_join<KIND>(acc);
-    if (threadIdx.x == 0) {
-        partials[tab.first_partial + b] = acc;
-        if (b == first && tab.step[t]) steps[tab.first_tensor + t] = *tab.step[t];
-    }
+    const double sum = group_join<KIND>(join<KIND>(acc[0], acc[1]));
+    if (threadIdx.x == 0) partials[tab.first_partial + blockIdx.x] = sum;
 }
 
 __global__ __launch_bounds__(kThreads) void norm_finish(Clip clip) {
@@ -167,16 +206,24 @@ __global__ __launch_bounds__(kThreads) void read_steps(StepTable tab, float* ste
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void scale_by_norm(ScaleTable tab, Clip clip) {
-    const int b = blockIdx.x;
-    const int t = find_tensor(tab.end, tab.n, b);
-    const int first = t ? tab.end[t - 1] : 0;
+    constexpr int V = 16 / sizeof(T), kStep = kThreads * V;
+    using P = Pack<T, V>;
     const double norm = norm_of(clip);
-    if (b == 0 && threadIdx.x == 0 && clip.norm) *clip.norm = (float)norm;
-    const float c = coefficient(norm, clip.max_norm);
-    T* g = (T*)tab.ptr[t];
-    const int64_t lo = (int64_t)(b - first) * tab.chunk;
-    const int64_t hi = lo + tab.chunk < tab.numel[t] ? lo + tab.chunk : tab.numel[t];
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) g[i] = (T)((float)g[i] * c);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = (float)norm;
+    const float s = coefficient(norm, clip.max_norm);
+    const int total = tab.end[tab.n - 1];
+    for (int b = blockIdx.x; b < total; b += gridDim.x) {
+        const Chunk c = find_chunk(tab, tab.end, b);
+        T* g = (T*)tab.ptr[c.t];
+        int64_t i = c.lo + threadIdx.x * V;
+        for (; i + V <= c.hi; i += kStep) {
+            typename P::type x = P::load(g + i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = (T)((float)x[j] * s);
+            P::store(g + i, x);
+        }
+        for (; i < c.hi; ++i) g[i] = (T)((float)g[i] * s);
+    }
 }
 
 // A 16-bit parameter is the rounding of its 32-bit master.  Left to itself the compiler forms the last multiply-add
@@ -184,47 +231,75 @@ __global__ __launch_bounds__(kThreads) void scale_by_norm(ScaleTable tab, Clip c
 // than the rounding of the rounded sum: the value has to exist in 32 bits first.
 __device__ __forceinline__ void keep_rounded(float& x) { asm("" : "+v"(x)); }
 
+struct Factors {
+    float clip, lr, inv1, inv2;     // inv1 = 1 / (1 - beta1^t), inv2 = 1 / sqrt(1 - beta2^t)
+};
+
+// One entry: its weight in 32 bits (the parameter itself, or its master), gradient and moments.
+__device__ __forceinline__ void adamw_entry(float& w, float g, float& m, float& v, const AdamArgs& a, const Factors& f) {
+    g *= f.clip;
+    m = a.beta1 * m + a.rest1 * g;
+    v = a.beta2 * v + a.rest2 * (g * g);
+    w -= f.lr * (m * f.inv1 / (sqrtf(v) * f.inv2 + a.eps) + a.decay * w);
+}
+
+// The weight that a step starts from.  The master stands for the parameter as long as it rounds to it: a parameter that
+// was written from outside (a loaded checkpoint) is taken as it is.
+template <typename T>
+__device__ __forceinline__ float weight_of(T p, float master) {
+    return (T)master == p ? master : (float)p;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adamw(AdamTable tab, Clip clip, AdamArgs a, const float* steps) {
     constexpr bool kMaster = sizeof(T) == 2;
-    const int b = blockIdx.x;
-    const int t = find_tensor(tab.end, tab.n, b);
-    const int first = t ? tab.end[t - 1] : 0;
-    float c = 1.f;
+    constexpr int V = 4, kStep = kThreads * V;
+    using P = Pack<T, V>;
+    using F = Pack<float, V>;
+    Factors f;
+    f.clip = 1.f;
     if (clip.partials) {
         const double norm = norm_of(clip);
-        if (b == 0 && tab.first_tensor == 0 && threadIdx.x == 0 && clip.norm) *clip.norm = (float)norm;
+        if (blockIdx.x == 0 && threadIdx.x == 0 && clip.norm) *clip.norm = (float)norm;
         if (clip.skip_nonfinite && !isfinite((float)norm)) return;
-        c = coefficient(norm, clip.max_norm);
+        f.clip = coefficient(norm, clip.max_norm);
     }
-    const float now = steps[tab.first_tensor + t] + 1.f;
-    if (b == first && threadIdx.x == 0) *tab.step[t] = now;
-    const float lr = a.lr_ptr ? *a.lr_ptr : a.lr;
-    const float inv1 = 1.f / -expm1f((float)(now * a.ln1));             // 1 / (1 - beta^t)
-    const float inv2 = 1.f / sqrtf(-expm1f((float)(now * a.ln2)));
-    T* p = (T*)tab.p[t];
-    const T* g = (const T*)tab.g[t];
-    float *m = tab.m[t], *v = tab.v[t], *w = tab.w[t];
-    const int64_t lo = (int64_t)(b - first) * tab.chunk;
-    const int64_t hi = lo + tab.chunk < tab.numel[t] ? lo + tab.chunk : tab.numel[t];
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
-        const float gi = (float)g[i] * c;
-        const float mi = a.beta1 * m[i] + a.rest1 * gi;
-        const float vi = a.beta2 * v[i] + a.rest2 * (gi * gi);
-        const T pi = p[i];
-        float wi = (float)pi;
-        if (kMaster) {
-            // the master stands for the parameter as long as it rounds to it: a parameter that was written from
-            // outside (a loaded checkpoint) is taken as it is
-            const float wm = w[i];
-            if ((T)wm == pi) wi = wm;
+    f.lr = a.lr_ptr ? *a.lr_ptr : a.lr;
+    const int total = tab.end[tab.n - 1];
+    for (int b = blockIdx.x; b < total; b += gridDim.x) {
+        const Chunk c = find_chunk(tab, tab.end, b);
+        const float now = steps[tab.id[c.t]] + 1.f;
+        if (c.first && threadIdx.x == 0) *tab.step[c.t] = now;
+        f.inv1 = 1.f / -expm1f((float)(now * a.ln1));
+        f.inv2 = 1.f / sqrtf(-expm1f((float)(now * a.ln2)));
+        T* p = (T*)tab.p[c.t];
+        const T* g = (const T*)tab.g[c.t];
+        float *m = tab.m[c.t], *v = tab.v[c.t], *w = tab.w[c.t];
+        int64_t i = c.lo + threadIdx.x * V;
+        for (; i + V <= c.hi; i += kStep) {
+            typename P::type pi = P::load(p + i);
+            const typename P::type gi = P::load(g + i);
+            typename F::type mi = F::load(m + i), vi = F::load(v + i), wi = {};
+            if (kMaster) wi = F::load(w + i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float wj = kMaster ? weight_of<T>(pi[j], wi[j]) : (float)pi[j], mj = mi[j], vj = vi[j];
+                adamw_entry(wj, (float)gi[j], mj, vj, a, f);
+                if (kMaster) keep_rounded(wj);
+                wi[j] = wj, mi[j] = mj, vi[j] = vj, pi[j] = (T)wj;
+            }
+            P::store(p + i, pi);
+            F::store(m + i, mi);
+            F::store(v + i, vi);
+            if (kMaster) F::store(w + i, wi);
         }
-        wi -= lr * (mi * inv1 / (sqrtf(vi) * inv2 + a.eps) + a.decay * wi);
-        if (kMaster) keep_rounded(wi);
-        m[i] = mi;
-        v[i] = vi;
-        p[i] = (T)wi;
-        if (kMaster) w[i] = wi;
+        for (; i < c.hi; ++i) {
+            float wi = kMaster ? weight_of<T>(p[i], w[i]) : (float)p[i], mi = m[i], vi = v[i];
+            adamw_entry(wi, (float)g[i], mi, vi, a, f);
+            if (kMaster) keep_rounded(wi);
+            m[i] = mi, v[i] = vi, p[i] = (T)wi;
+            if (kMaster) w[i] = wi;
+        }
     }
 }
 
@@ -273,67 +348,88 @@ int check_disjoint(void* const* ptr, const int64_t* numel, const int32_t* dtype,
     return apart ? NERF_OK : NERF_ERR_ARG;
 }
 
-// Elements per chunk: as few as kMinChunk while the list is short (latency: every compute unit gets some), more once
-// there would be more than kMaxPartials chunks.
-int64_t chunk_for(const int64_t* numel, int n) {
+// Elements per chunk: as few as kMinChunk while the list is short (latency: every compute unit gets some), up to
+// kMaxChunk for a long one (a chunk's lookup is paid once per kMaxChunk elements), more only where 2^30 chunks would not
+// do.
+int chunk_for(const int64_t* numel, int n) {
     int64_t total = 0;
     for (int i = 0; i < n; ++i) total += numel[i];
     int64_t chunk = kMinChunk;
-    while ((total + chunk - 1) / chunk > kMaxPartials) chunk *= 2;
-    return chunk;
+    while ((chunk < kMaxChunk && total / chunk > kMaxGroups) || total / chunk > ((int64_t)1 << 30)) chunk *= 2;
+    return (int)chunk;
 }
 
+int groups_for(int chunks) { return chunks < kMaxGroups ? chunks : kMaxGroups; }
+
 // a tensor without elements has one empty chunk (its step counter still counts)
-int chunks_of(int64_t numel, int64_t chunk) { return numel ? (int)((numel + chunk - 1) / chunk) : 1; }
+int chunks_of(int64_t numel, int chunk) { return numel ? (int)((numel + chunk - 1) / chunk) : 1; }
+
+// A launch leaves at most kMaxGroups partials, and there are as many launches as full tables and one more per type.
+int64_t max_partials(int n) { return (int64_t)kMaxGroups * (3 + n / kNormCap); }
 
 struct Workspace {
     double* partials;
     float* steps;
 };
 
-int64_t workspace_bytes(int n) { return (int64_t)(kMaxPartials + n) * 8 + (int64_t)n * 4; }
+int64_t workspace_bytes(int n) { return max_partials(n) * 8 + (int64_t)n * 4; }
 
 int take_workspace(void* ws, int64_t bytes, int n, Workspace* out) {
     NERF_REQUIRE(ws && (uintptr_t)ws % 8 == 0 && bytes >= workspace_bytes(n));
     out->partials = (double*)ws;
-    out->steps = (float*)(out->partials + kMaxPartials + n);
+    out->steps = (float*)(out->partials + max_partials(n));
     return NERF_OK;
 }
 
-template <typename T>
-void launch_norm(const NormTable& tab, int kind, const Workspace& ws, hipStream_t st) {
-    const dim3 grid(tab.end[tab.n - 1]), block(kThreads);
-    if (kind == NERF_NORM_L2) norm_partials<T, NERF_NORM_L2><<<grid, block, 0, st>>>(tab, ws.partials, ws.steps);
-    else if (kind == NERF_NORM_L1) norm_partials<T, NERF_NORM_L1><<<grid, block, 0, st>>>(tab, ws.partials, ws.steps);
-    else norm_partials<T, NERF_NORM_MAX><<<grid, block, 0, st>>>(tab, ws.partials, ws.steps);
+constexpr int kDtypes[] = {NERF_F32, NERF_BF16, NERF_F16};
+
+// fill(k, i) puts tensor i into place k of a table; go(d) launches a full one, and the last of each type.
+template <typename Table, int CAP, typename Fill, typename Go>
+void for_tables(Table& tab, int (&ends)[CAP], const int64_t* numel, const int32_t* dtype, int first, int last, Fill fill, Go go) {
+    for (int d : kDtypes) {
+        tab.n = 0;
+        int end = 0;
+        for (int i = first; i < last; ++i) {
+            if (dtype[i] != d) continue;
+            end += chunks_of(numel[i], tab.chunk);
+            fill(tab.n, i);
+            tab.numel[tab.n] = numel[i];
+            ends[tab.n] = end;
+            if (++tab.n == CAP) {
+                go(d, groups_for(end));
+                tab.n = end = 0;
+            }
+        }
+        if (tab.n) go(d, groups_for(end));
+    }
 }
 
-// The norm's first launch(es): a partial per chunk.  Tables hold consecutive tensors of one type.
+template <typename T>
+void launch_norm(const NormTable& tab, int grid, int kind, const Workspace& ws, hipStream_t st) {
+    if (kind == NERF_NORM_L2) norm_partials<T, NERF_NORM_L2><<<grid, kThreads, 0, st>>>(tab, ws.partials, ws.steps);
+    else if (kind == NERF_NORM_L1) norm_partials<T, NERF_NORM_L1><<<grid, kThreads, 0, st>>>(tab, ws.partials, ws.steps);
+    else norm_partials<T, NERF_NORM_MAX><<<grid, kThreads, 0, st>>>(tab, ws.partials, ws.steps);
+}
+
+// The norm's first launch(es): a partial per workgroup.
 int run_norm(const void* const* ptr, float* const* step, const int64_t* numel, const int32_t* dtype, int n, int kind,
              const Workspace& ws, int* n_partials, hipStream_t st) {
-    const int64_t chunk = chunk_for(numel, n);
     NormTable tab;
-    tab.chunk = chunk;
-    int partials = 0;
-    for (int i = 0; i < n;) {
-        const int d = dtype[i];
-        tab.n = 0;
-        tab.first_tensor = i;
-        tab.first_partial = partials;
-        int end = 0;
-        for (; i < n && tab.n < kNormCap && dtype[i] == d; ++i, ++tab.n) {
-            end += chunks_of(numel[i], chunk);
-            tab.ptr[tab.n] = ptr[i];
-            tab.step[tab.n] = step ? step[i] : nullptr;
-            tab.numel[tab.n] = numel[i];
-            tab.end[tab.n] = end;
-        }
-        partials += end;
-        if (d == NERF_F32) launch_norm<float>(tab, kind, ws, st);
-        else if (d == NERF_BF16) launch_norm<__bf16>(tab, kind, ws, st);
-        else launch_norm<_Float16>(tab, kind, ws, st);
-    }
-    *n_partials = partials;
+    tab.chunk = chunk_for(numel, n);
+    tab.first_partial = 0;
+    for_tables(tab, tab.end, numel, dtype, 0, n,
+               [&](int k, int i) {
+                   tab.ptr[k] = ptr[i];
+                   tab.step[k] = step ? step[i] : nullptr;
+                   tab.id[k] = i;
+               },
+               [&](int d, int grid) {
+                   if (d == NERF_F32) launch_norm<float>(tab, grid, kind, ws, st);
+                   else if (d == NERF_BF16) launch_norm<__bf16>(tab, grid, kind, ws, st);
+                   else launch_norm<_Float16>(tab, grid, kind, ws, st);
+                   tab.first_partial += grid;
+               });
+    *n_partials = tab.first_partial;
     return nerf_launch_status();
 }
 
@@ -371,20 +467,12 @@ extern "C" int nerf_clip_grad_norm(void* const* grads, const int64_t* numel, con
     }
     ScaleTable tab;
     tab.chunk = chunk_for(numel, n_tensors);
-    for (int i = 0; i < n_tensors;) {
-        const int d = dtype[i];
-        int end = 0;
-        tab.n = 0;
-        for (; i < n_tensors && tab.n < kScaleCap && dtype[i] == d; ++i, ++tab.n) {
-            end += chunks_of(numel[i], tab.chunk);
-            tab.ptr[tab.n] = grads[i];
-            tab.numel[tab.n] = numel[i];
-            tab.end[tab.n] = end;
-        }
-        if (d == NERF_F32) scale_by_norm<float><<<end, kThreads, 0, st>>>(tab, clip);
-        else if (d == NERF_BF16) scale_by_norm<__bf16><<<end, kThreads, 0, st>>>(tab, clip);
-        else scale_by_norm<_Float16><<<end, kThreads, 0, st>>>(tab, clip);
-    }
+    for_tables(tab, tab.end, numel, dtype, 0, n_tensors, [&](int k, int i) { tab.ptr[k] = grads[i]; },
+               [&](int d, int grid) {
+                   if (d == NERF_F32) scale_by_norm<float><<<grid, kThreads, 0, st>>>(tab, clip);
+                   else if (d == NERF_BF16) scale_by_norm<__bf16><<<grid, kThreads, 0, st>>>(tab, clip);
+                   else scale_by_norm<_Float16><<<grid, kThreads, 0, st>>>(tab, clip);
+               });
     return nerf_launch_status();
 }
 
@@ -436,32 +524,27 @@ extern "C" int nerf_adamw_step(const nerf_adamw_tensors* t, const nerf_adamw_gro
     }
     AdamTable tab;
     tab.chunk = chunk_for(t->numel, n);
-    int i = 0, group_end = 0;
+    int first = 0;
     for (int k = 0; k < n_groups; ++k) {
         const nerf_adamw_group& g = groups[k];
-        group_end += g.count;
         const AdamArgs a{g.lr_device, (float)g.lr, (float)g.beta2, (float)g.eps, (float)g.weight_decay, (float)(1.0 - g.beta1),
                          (float)(1.0 - g.beta2), (float)g.beta1, log(g.beta1), log(g.beta2)};
-        while (i < group_end) {
-            const int d = t->dtype[i];
-            int end = 0;
-            tab.n = 0;
-            tab.first_tensor = i;
-            for (; i < group_end && tab.n < kAdamCap && t->dtype[i] == d; ++i, ++tab.n) {
-                end += chunks_of(t->numel[i], tab.chunk);
-                tab.p[tab.n] = t->param[i];
-                tab.g[tab.n] = t->grad[i];
-                tab.m[tab.n] = t->exp_avg[i];
-                tab.v[tab.n] = t->exp_avg_sq[i];
-                tab.w[tab.n] = t->master ? t->master[i] : nullptr;
-                tab.step[tab.n] = t->step[i];
-                tab.numel[tab.n] = t->numel[i];
-                tab.end[tab.n] = end;
-            }
-            if (d == NERF_F32) adamw<float><<<end, kThreads, 0, st>>>(tab, clip, a, ws.steps);
-            else if (d == NERF_BF16) adamw<__bf16><<<end, kThreads, 0, st>>>(tab, clip, a, ws.steps);
-            else adamw<_Float16><<<end, kThreads, 0, st>>>(tab, clip, a, ws.steps);
-        }
+        for_tables(tab, tab.end, t->numel, t->dtype, first, first + g.count,
+                   [&](int j, int i) {
+                       tab.p[j] = t->param[i];
+                       tab.g[j] = t->grad[i];
+                       tab.m[j] = t->exp_avg[i];
+                       tab.v[j] = t->exp_avg_sq[i];
+                       tab.w[j] = t->master ? t->master[i] : nullptr;
+                       tab.step[j] = t->step[i];
+                       tab.id[j] = i;
+                   },
+                   [&](int d, int grid) {
+                       if (d == NERF_F32) adamw<float><<<grid, kThreads, 0, st>>>(tab, clip, a, ws.steps);
+                       else if (d == NERF_BF16) adamw<__bf16><<<grid, kThreads, 0, st>>>(tab, clip, a, ws.steps);
+                       else adamw<_Float16><<<grid, kThreads, 0, st>>>(tab, clip, a, ws.steps);
+                   });
+        first += g.count;
     }
     return nerf_launch_status();
 }
