@@ -24,8 +24,9 @@ class MlpDims(Structure):
 
 
 class AdamwTensors(Structure):
-    _fields_ = [('n_tensors', c_int), ('param', c_void_p), ('grad', c_void_p), ('exp_avg', c_void_p),
-                ('exp_avg_sq', c_void_p), ('master', c_void_p), ('step', c_void_p), ('numel', c_void_p), ('dtype', c_void_p)]
+    # (c_char_p: the arrays come as bytes objects, which the structure then keeps alive)
+    _fields_ = [('n_tensors', c_int), ('param', c_char_p), ('grad', c_char_p), ('exp_avg', c_char_p),
+                ('exp_avg_sq', c_char_p), ('master', c_char_p), ('step', c_char_p), ('numel', c_char_p), ('dtype', c_char_p)]
 
 
 class AdamwGroup(Structure):
@@ -114,6 +115,26 @@ def check(code):
 
 def stream():
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_lists = None
+
+
+def lists():
+    """The host module that reads lists of tensors (csrc/tensor_lists.cpp)."""
+    global _lists
+    if _lists is None:
+        try:
+            from . import _tensor_lists
+        except ImportError as e:
+            raise ImportError(f'nerf_amd._tensor_lists: {e} (build it with `python -m nerf_amd.build`)') from None
+        _lists = _tensor_lists
+    return _lists
+
+
+def raw_stream(device_index):
+    """Handle of a device's current stream, as `stream()` without the Stream object around it."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def ptr(t, dtype=torch.float32):

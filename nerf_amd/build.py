@@ -1,4 +1,4 @@
-"""Build libnerf_amd.so (gfx950) in-tree with hipcc.
+"""Build libnerf_amd.so (gfx950) in-tree with hipcc, and the host module that reads tensor lists (`_tensor_lists`).
 
     python -m nerf_amd.build [--force]
 
@@ -34,6 +34,8 @@ UNITS = {
     'wgrad8.o': ('wgrad8.hip', ['-mllvm', '-amdgpu-mfma-vgpr-form']),
 }
 UNITS.update({'mlp_bf16_p%d.o' % p: ('mlp_bf16.hip', ['-DNERF_NET_PART=%d' % p]) for p in range(8)})   # default contraction
+LISTS_SRC = os.path.join(CSRC, 'tensor_lists.cpp')
+LISTS = os.path.join(HERE, '_tensor_lists.so')
 JOBS = int(os.environ.get('MAX_JOBS', '8'))
 
 
@@ -51,6 +53,18 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _lists_command():
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    libdir = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    return (['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall',
+             '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch.compiled_with_cxx11_abi()]
+            + ['-I' + d for d in include_paths() + [sysconfig.get_paths()['include']]]
+            + [LISTS_SRC, '-o', LISTS, '-L' + libdir, '-ltorch_python', '-ltorch_cpu', '-lc10'])
+
+
 def build(force=False, verbose=True):
     os.makedirs(OBJDIR, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(('.h', '.inc'))]
@@ -63,6 +77,7 @@ def build(force=False, verbose=True):
         objs.append(obj)
         if force or _stale(obj, [src] + headers):
             jobs.append([_hipcc()] + COMMON + extra + ['-c', src, '-o', obj])
+    host = [_lists_command()] if force or _stale(LISTS, [LISTS_SRC, os.path.abspath(__file__)]) else []
     for f in os.listdir(OBJDIR):                      # objects of an older unit list must not be linked
         if f.endswith('.o') and f not in UNITS:
             os.remove(os.path.join(OBJDIR, f))
@@ -72,8 +87,8 @@ def build(force=False, verbose=True):
             print(' '.join(cmd), flush=True)
         subprocess.run(cmd, check=True)
 
-    with ThreadPoolExecutor(max_workers=min(JOBS, max(1, len(jobs)))) as ex:
-        list(ex.map(run, jobs))
+    with ThreadPoolExecutor(max_workers=min(JOBS, max(1, len(jobs + host)))) as ex:
+        list(ex.map(run, jobs + host))
     if jobs or force or _stale(LIB, objs):
         run([_hipcc(), '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB] + objs)
     return LIB

@@ -5,7 +5,6 @@ reference-compatible surface lives in `nerf_amd.utils`.
 """
 import ctypes
 import math
-from array import array
 
 import torch
 
@@ -265,7 +264,6 @@ def sar_pulse_loss(pulse, mfilt, target, coarse_weight, need_grad=True, need_pro
 
 # ---- gradient norm, clipping, optimizer step over a list of tensors (csrc/optimizer.hip) ----------------------------
 
-LIST_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 NORM_KINDS = {1.0: 1, 2.0: 2, math.inf: 3}
 
 
@@ -284,59 +282,27 @@ def check_max_norm(max_norm):
     return max_norm
 
 
-def list_device(tensors):
-    """The index of the one HIP device that holds every tensor of a list."""
-    devices = {t.get_device() for t in tensors}
-    if len(devices) > 1:
-        raise RuntimeError('nerf_amd kernels need the tensors of a list on one HIP device')
-    dev = devices.pop()
-    if dev < 0:
-        raise RuntimeError('nerf_amd kernels need tensors on a HIP device; got a CPU tensor')
-    return dev
+def list_call(device, call):
+    """call(stream handle) with `device` (an index) the current one."""
+    if device == torch.cuda.current_device():
+        return call(_lib.raw_stream(device))
+    with torch.cuda.device(device):
+        return call(_lib.raw_stream(device))
 
 
-def list_dtypes(tensors):
-    try:
-        return array('i', [LIST_DTYPES[t.dtype] for t in tensors])
-    except KeyError as e:
-        raise RuntimeError(f'expected float32, bfloat16 or float16 tensors, got {e.args[0]}') from None
-
-
-def is_dense(t):
-    """Whether the entries of `t` fill a stretch of memory without gaps or overlaps, in whatever order."""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-def _addr(a):
-    return a.buffer_info()[0]
-
-
-def ptr_array(tensors):
-    return array('Q', [t.data_ptr() for t in tensors])
-
-
-def _list_call(entry, tensors, *args):
-    """entry(pointers, numels, dtypes, n, *args, workspace, bytes, norm, stream) on the device that holds the list
-    -> the norm, a 0-d fp32 tensor."""
+def _norm_call(entry, tensors, table, *args):
+    """entry(pointers, numels, dtypes, n, *args, workspace, bytes, norm, stream) on the list's device -> the norm, a 0-d
+    fp32 tensor."""
     n = len(tensors)
-    dev = list_device(tensors) if n else torch.cuda.current_device()
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _list_call(entry, tensors, *args)
-    ptrs, dtypes = ptr_array(tensors), list_dtypes(tensors)
-    numels = array('q', [t.numel() for t in tensors])
-    nbytes = lib().nerf_grad_workspace_bytes(n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device='cuda')
-    norm = torch.empty((), dtype=torch.float32, device='cuda')
-    check(entry(_addr(ptrs), _addr(numels), _addr(dtypes), n, *args, ws.data_ptr(), nbytes, norm.data_ptr(), stream()))
-    return norm
+    device, ptrs, numels, dtypes, _ = table
+
+    def call(st):
+        nbytes = lib().nerf_grad_workspace_bytes(n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device='cuda')
+        norm = torch.empty((), dtype=torch.float32, device='cuda')
+        check(entry(ptrs, numels, dtypes, n, *args, ws.data_ptr(), nbytes, norm.data_ptr(), st))
+        return norm
+    return list_call(device if n else torch.cuda.current_device(), call)
 
 
 def _as_list(tensors):
@@ -349,9 +315,11 @@ def grad_norm(tensors, norm_type=2.0):
     in 64 bits and added in a fixed order.  A NaN entry gives NaN; an empty list gives 0.  No gradient flows through it."""
     kind = norm_kind(norm_type)
     tensors = _as_list(tensors)
-    if not all(t.is_contiguous() for t in tensors):     # any dense order will do; anything else is copied
-        tensors = [t if is_dense(t) else t.detach().contiguous() for t in tensors]
-    return _list_call(lib().nerf_grad_norm, tensors, kind)
+    table = _lib.lists().describe(tensors)
+    if not table[-1]:           # any dense order will do; anything else is copied
+        tensors = [t if _lib.lists().is_dense(t) else t.detach().contiguous() for t in tensors]
+        table = _lib.lists().describe(tensors)
+    return _norm_call(lib().nerf_grad_norm, tensors, table, kind)
 
 
 def clip_grad_norm_(tensors, max_norm, norm_type=2.0):
@@ -361,8 +329,9 @@ def clip_grad_norm_(tensors, max_norm, norm_type=2.0):
     must be dense (any order of dimensions) and must not share memory."""
     kind, max_norm = norm_kind(norm_type), check_max_norm(max_norm)
     tensors = _as_list(tensors)
-    if not all(t.is_contiguous() or is_dense(t) for t in tensors):
+    table = _lib.lists().describe(tensors)
+    if not table[-1]:
         raise RuntimeError('clip_grad_norm_: expected dense tensors (no gaps, no broadcast dimensions)')
-    norm = _list_call(lib().nerf_clip_grad_norm, tensors, kind, max_norm)
+    norm = _norm_call(lib().nerf_clip_grad_norm, tensors, table, kind, max_norm)
     torch.autograd.graph.increment_version(tensors)     # (the kernels write behind autograd's back)
     return norm

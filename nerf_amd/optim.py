@@ -7,14 +7,11 @@ parameters together, takes the gradients' norm and clips them while it reads the
 The tensor-level entry points are `nerf_amd.ops.grad_norm` and `nerf_amd.ops.clip_grad_norm_`.
 """
 import ctypes
-from array import array
 
 import torch
 
 from . import ops
-from ._lib import AdamwGroup, AdamwTensors, check, lib, stream
-
-_addr = ops._addr
+from ._lib import AdamwGroup, AdamwTensors, check, lib, lists
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -89,85 +86,88 @@ class AdamW(torch.optim.Optimizer):
                     del g[k]
             g['capturable'] = True
 
-    def _init_state(self, params):
+    @staticmethod
+    def _not_captured():
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('AdamW: run one step ahead of a graph capture (it lays out the optimizer state; captured, '
                                'every replay would clear it)')
+
+    def _master_of(self, p):
+        self._not_captured()
+        return p.detach().to(torch.float32, memory_format=torch.preserve_format)
+
+    def _init_state(self, params):
+        self._not_captured()
         steps = torch.zeros(len(params), dtype=torch.float32, device=params[0].device)
         for i, p in enumerate(params):
             st = self.state[p]
             st['step'] = steps[i]
             st['exp_avg'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
             st['exp_avg_sq'] = torch.zeros_like(st['exp_avg'])
+            if p.dtype != torch.float32:
+                st['master'] = self._master_of(p)
 
-    def _check_state(self, p, st):
-        """State that came from outside has to be what the kernel reads: fp32, on the device, laid out as the parameter."""
-        for k in ('exp_avg', 'exp_avg_sq', 'master'):
-            t = st.get(k)
-            if t is not None and (t.dtype != torch.float32 or t.get_device() != p.get_device() or t.shape != p.shape
-                                  or not (t.stride() == p.stride() or t.is_contiguous() and p.is_contiguous())):
-                raise RuntimeError(f'AdamW: state {k!r} must be an fp32 tensor of the parameter\'s shape, order and device')
-        t = st['step']
-        if t.dtype != torch.float32 or t.get_device() != p.get_device() or t.numel() != 1:
-            raise RuntimeError('AdamW: state \'step\' must be one fp32 number on the parameter\'s device')
-
-    def _grad_of(self, p):
-        g = p.grad
-        if g.is_sparse or g.dtype != p.dtype or g.get_device() != p.get_device():
-            raise RuntimeError('AdamW: gradients must be dense tensors of their parameters\' type and device')
-        if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
-            # another order of the same entries: laid out as the parameter is
-            g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
-        return g
-
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        params, counts = [], []
+        params, grads, counts = [], [], []
         for group in self.param_groups:
-            with_grad = [p for p in group['params'] if p.grad is not None]
-            counts.append(len(with_grad))
-            params += with_grad
+            before = len(params)
+            for p in group['params']:
+                g = p.grad
+                if g is not None:
+                    params.append(p)
+                    grads.append(g)
+            counts.append(len(params) - before)
         clips = self.max_norm is not None or self.skip_nonfinite
-        if not params:
-            if clips:
-                p = next((p for g in self.param_groups for p in g['params']), None)
-                self.grad_norm = torch.zeros((), device=p.device if p is not None else None)
-            return loss
-        dev = ops.list_device(params)
-        if dev != torch.cuda.current_device():
-            with torch.cuda.device(dev):
-                self._step(params, counts, clips)
-        else:
-            self._step(params, counts, clips)
+        if params:
+            table = lists().describe(params)
+            if not table[-1]:
+                raise RuntimeError('AdamW: expected dense parameters (no gaps, no broadcast dimensions)')
+            ops.list_call(table[0], lambda st: self._launch(params, grads, counts, clips, table, st))
+            torch.autograd.graph.increment_version(params)      # (the kernels write behind autograd's back)
+        elif clips:
+            p = next((p for g in self.param_groups for p in g['params']), None)
+            self.grad_norm = torch.zeros((), device=p.device if p is not None else None)
         return loss
 
-    def _step(self, params, counts, clips):
-        dtypes = ops.list_dtypes(params)
-        for p in params:
-            if not (p.is_contiguous() or ops.is_dense(p)):
-                raise RuntimeError('AdamW: expected dense parameters')
-        grads = [self._grad_of(p) for p in params]
-        fresh = [p for p in params if 'exp_avg' not in self.state[p]]
-        if fresh:
-            self._init_state(fresh)
+    def _states(self, params, half):
         states = [self.state[p] for p in params]
-        half = any(dtypes)
+        if {} in states:
+            self._init_state([p for p, st in zip(params, states) if not st])
         if half:
             for p, st in zip(params, states):
-                if p.dtype != torch.float32 and 'master' not in st:
-                    st['master'] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
-        for p, st in zip(params, states):
-            self._check_state(p, st)
+                if 'master' not in st and p.dtype != torch.float32:     # (the state of an optimizer that keeps none)
+                    st['master'] = self._master_of(p)
+        return states
+
+    @torch.no_grad()
+    def _as_params(self, tensors, params):
+        """The tensors laid out as their parameters are (another order of the same entries)."""
+        return [torch.empty_like(p, memory_format=torch.preserve_format).copy_(t) for t, p in zip(tensors, params)]
+
+    def _launch(self, params, grads, counts, clips, table, st):
+        L, match = lib(), lists().match
         n = len(params)
-        arrays = [ops.ptr_array(params), ops.ptr_array(grads), ops.ptr_array([s['exp_avg'] for s in states]),
-                  ops.ptr_array([s['exp_avg_sq'] for s in states]),
-                  array('Q', [s['master'].data_ptr() if 'master' in s else 0 for s in states]),
-                  ops.ptr_array([s['step'] for s in states]), array('q', [p.numel() for p in params]), dtypes]
-        table = AdamwTensors(n, *(_addr(a) for a in arrays))
+        device, ptrs, numels, dtypes, _ = table
+        grad_ptrs = match(grads, params, False)
+        if grad_ptrs is None:
+            grads = self._as_params(grads, params)
+            grad_ptrs = match(grads, params, False)
+        states = self._states(params, dtypes.strip(b'\0'))
+        state_ptrs = []
+        for k in ('exp_avg', 'exp_avg_sq', 'master'):
+            found = match([s.get(k) for s in states], params, True)
+            if found is None:
+                raise RuntimeError(f'AdamW: state {k!r} has another order of dimensions than its parameter')
+            state_ptrs.append(found)
+        step_device, step_ptrs, _, step_types, _ = lists().describe([s['step'] for s in states])
+        if step_device != device or step_types.strip(b'\0'):
+            raise RuntimeError('AdamW: state \'step\' must be fp32 on the parameters\' device')
+        arrays = (ptrs, grad_ptrs, *state_ptrs, step_ptrs, numels, dtypes)
+        t = AdamwTensors(n, *arrays)
         groups = (AdamwGroup * len(counts))()
         for c, count, g in zip(groups, counts, self.param_groups):
             lr = g['lr']
@@ -176,7 +176,7 @@ class AdamW(torch.optim.Optimizer):
                 if lr.numel() != 1:
                     raise ValueError('AdamW: a tensor learning rate must have one element')
                 if lr.is_cuda:
-                    if lr.dtype != torch.float32 or lr.get_device() != params[0].get_device():
+                    if lr.dtype != torch.float32 or lr.get_device() != device:
                         raise ValueError('AdamW: a tensor learning rate must be fp32 on the parameters\' device')
                     c.lr_device = lr.data_ptr()
                 else:
@@ -185,13 +185,11 @@ class AdamW(torch.optim.Optimizer):
                 c.lr = float(lr)
             c.beta1, c.beta2 = g['betas']
             c.eps, c.weight_decay = g['eps'], g['weight_decay']
-        nbytes = lib().nerf_grad_workspace_bytes(n)
+        nbytes = L.nerf_grad_workspace_bytes(n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device='cuda')
         norm = torch.empty((), dtype=torch.float32, device='cuda') if clips else None
-        max_norm = float('inf') if self.max_norm is None else self.max_norm
-        check(lib().nerf_adamw_step(ctypes.byref(table), groups, len(counts), self._kind if clips else 0, max_norm,
-                                    int(self.skip_nonfinite), ws.data_ptr(), nbytes, norm.data_ptr() if clips else None,
-                                    stream()))
+        check(L.nerf_adamw_step(ctypes.byref(t), groups, len(counts), self._kind if clips else 0,
+                                float('inf') if self.max_norm is None else self.max_norm, int(self.skip_nonfinite),
+                                ws.data_ptr(), nbytes, norm.data_ptr() if clips else None, st))
         if clips:
             self.grad_norm = norm
-        torch.autograd.graph.increment_version(params)      # (the kernels write behind autograd's back)

@@ -207,11 +207,18 @@ def test_refusals_on_the_device():
         opt.step()
     opt = optim.AdamW([p])
     opt.state[p] = dict(step=torch.zeros(()), exp_avg=torch.zeros_like(p), exp_avg_sq=torch.zeros_like(p))
-    with pytest.raises(RuntimeError, match='step'):
+    with pytest.raises(RuntimeError, match='HIP device'):
         opt.step()
     opt.state[p] = dict(step=torch.zeros((), device='cuda'), exp_avg=torch.zeros(4), exp_avg_sq=torch.zeros_like(p))
-    with pytest.raises(RuntimeError, match='exp_avg'):
+    with pytest.raises(RuntimeError, match='shape and device'):
         opt.step()
+    opt.state[p] = dict(step=torch.zeros((), device='cuda', dtype=torch.bfloat16), exp_avg=torch.zeros_like(p),
+                        exp_avg_sq=torch.zeros_like(p))
+    with pytest.raises(RuntimeError, match='step'):
+        opt.step()
+    for t in (torch.zeros(4, 6, device='cuda')[:, :3], torch.zeros(1, 3, device='cuda').expand(4, 3)):
+        with pytest.raises(RuntimeError, match='dense'):
+            ops.clip_grad_norm_([x, t], 1.0)
     q = torch.nn.Parameter(torch.zeros(4, 6, device='cuda')[:, :3])
     q.grad = torch.zeros_like(q)
     with pytest.raises(RuntimeError, match='dense'):
@@ -537,13 +544,12 @@ def test_captured_clip():
 
 
 def test_the_c_entries_allocate_nothing_and_need_no_stream():
-    from nerf_amd import _lib, ops
+    from nerf_amd import _lib
     t = make([100_001], torch.float32)[0]
     L = _lib.lib()
-    ptrs, numels, dtypes = ops.ptr_array([t]), ops.array('q', [t.numel()]), ops.list_dtypes([t])
+    args = _lib.lists().describe([t])[1:4]
     n = L.nerf_grad_workspace_bytes(1)
     ws, norm = torch.empty(n, dtype=torch.uint8, device='cuda'), torch.empty((), device='cuda')
-    args = [a.buffer_info()[0] for a in (ptrs, numels, dtypes)]
     torch.cuda.synchronize()
     assert L.nerf_grad_norm(*args, 1, 2, ws.data_ptr(), n, norm.data_ptr(), ctypes.c_void_p(None)) == 0
     torch.cuda.synchronize()

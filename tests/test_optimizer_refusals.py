@@ -117,12 +117,6 @@ def test_host_tensors():
     assert torch.equal(p.detach(), CPU) and torch.equal(p.grad, torch.ones(8))
 
 
-@pytest.mark.parametrize('t', [torch.zeros(4, 6)[:, :3], torch.zeros(1, 3).expand(4, 3), torch.zeros(9)[::2]])
-def test_clip_needs_dense_tensors(t):
-    with pytest.raises(RuntimeError, match='dense'):
-        ops.clip_grad_norm_([t], 1.0)
-
-
 @pytest.mark.parametrize('t,dense', [
     (torch.zeros(4, 6).t(), True), (torch.zeros(2, 3, 4).permute(2, 0, 1), True), (torch.zeros(1, 5)[:, ::1], True),
     (torch.zeros(2, 3, 4, 5).contiguous(memory_format=torch.channels_last), True), (torch.zeros(0, 3).t(), True),
@@ -130,7 +124,32 @@ def test_clip_needs_dense_tensors(t):
     (torch.zeros(5, 1).expand(5, 1).t(), True), (torch.zeros(6, 4)[::2].t(), False),
 ])
 def test_is_dense(t, dense):
-    assert ops.is_dense(t) is dense
+    assert _lib.lists().is_dense(t) is dense
+
+
+def test_list_reader():
+    L = _lib.lists()
+    for bad in (CPU, (CPU,), [3], [None], None):
+        with pytest.raises(TypeError):
+            L.describe(bad)
+    assert L.describe([]) == (-1, b'', b'', b'', True)
+    with pytest.raises(RuntimeError, match='HIP device'):
+        L.describe([CPU])
+    with pytest.raises(RuntimeError, match='strided'):
+        L.describe([torch.zeros(3, 3).to_sparse()])
+    with pytest.raises(RuntimeError, match='strided'):
+        L.describe([torch.zeros(3, dtype=torch.complex64).conj().imag])
+    a, b = torch.zeros(3, 4), torch.zeros(4, 3).t()
+    read = lambda x: array('Q', x).tolist()         # noqa: E731
+    assert read(L.match([a, None], [a, b], False)) == [a.data_ptr(), 0]
+    assert read(L.match([torch.zeros(1, 5).t().contiguous().t()], [torch.zeros(1, 5)], False)) != [0]
+    assert L.match([a], [b], False) is None
+    assert L.match([b], [b], True) is not None
+    for x, y, fp32 in ((a, torch.zeros(4, 3), False), (a.half(), a, False), (a.half(), a.half(), True)):
+        with pytest.raises(RuntimeError, match='shape'):
+            L.match([x], [y], fp32)
+    with pytest.raises(ValueError):
+        L.match([a], [], False)
 
 
 def test_unsupported_optimizer_states():
