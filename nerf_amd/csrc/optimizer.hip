@@ -16,49 +16,59 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kNormCap = 112;       // tensors per launch: the tables stay below 4 KB of kernel arguments
-constexpr int kScaleCap = 176;
-constexpr int kAdamCap = 56;
+
+// How a kernel's launches are cut: at most `groups` workgroups, and chunks of `least` elements (one access per lane) while
+// the list is short, so that every compute unit gets some, up to `most` for a long one.
+struct Cut {
+    int groups, least, most;
+};
+constexpr int kNormGroups = 1024;
+constexpr Cut norm_cut(int size) { return {kNormGroups, 4096 / size, 32768 / size}; }
+constexpr Cut scale_cut(int size) { return {1024, 4096 / size, 16384 / size}; }
+constexpr Cut adam_cut(int) { return {768, 1024, 4096}; }
+
+constexpr int64_t kMiB = 1 << 20;
+constexpr int64_t kNormStream = 64 * kMiB;
+constexpr int64_t kUpdateStream = 192 * kMiB;
+
+// The tables stay below 4 KB of kernel arguments.  A tensor's chunks are counted from the start of the line of memory that
+// holds its first element (`shift` elements before it), so that a wave's accesses cover whole lines but at the two ends.
+template <int CAP>
+struct Chunks {
+    static constexpr int kCap = CAP;
+    int end[CAP];           // chunks of the tensors up to and including this one
+    int tail[CAP];          // elements of its last chunk (with `shift` where that is its first one too)
+    int n, chunk;
+};
+
+struct ListTable : Chunks<224> {
+    void* ptr[kCap];
+};
+
+struct NormStepTable : Chunks<120> {    // with the step counters, which the norm's launch copies to the workspace
+    void* ptr[kCap];
+    const float* step[kCap];
+    int id[kCap];           // place in the caller's list
+};
+
+struct AdamTable : Chunks<56> {
+    void* p[kCap];
+    const void* g[kCap];
+    float* m[kCap];
+    float* v[kCap];
+    float* w[kCap];         // 32-bit master weights (16-bit parameters)
+    float* step[kCap];
+    int id[kCap];
+};
+
 constexpr int kStepCap = 256;
-constexpr int kMaxGroups = 2048;    // workgroups of one launch: eight per compute unit
-constexpr int kMinChunk = 1024;
-constexpr int kMaxChunk = 16384;
-
-struct NormTable {
-    const void* ptr[kNormCap];
-    const float* step[kNormCap];    // null, or the tensor's step counter: copied to the workspace
-    int64_t numel[kNormCap];
-    int end[kNormCap];              // chunks of the tensors up to and including this one
-    int id[kNormCap];               // place in the caller's list
-    int n, first_partial, chunk;
-};
-
-struct ScaleTable {
-    void* ptr[kScaleCap];
-    int64_t numel[kScaleCap];
-    int end[kScaleCap];
-    int n, chunk;
-};
-
-struct AdamTable {
-    void* p[kAdamCap];
-    const void* g[kAdamCap];
-    float* m[kAdamCap];
-    float* v[kAdamCap];
-    float* w[kAdamCap];             // 32-bit master weights (16-bit parameters)
-    float* step[kAdamCap];
-    int64_t numel[kAdamCap];
-    int end[kAdamCap];
-    int id[kAdamCap];
-    int n, chunk;
-};
-
 struct StepTable {
     const float* step[kStepCap];
     int n, first_tensor;
@@ -73,46 +83,65 @@ struct Clip {
 
 struct AdamArgs {
     const float* lr_ptr;            // null: lr
-    float lr, beta2, eps, decay, rest1, rest2;      // rest = 1 - beta, rounded from 64 bits
-    float beta1;
+    float lr, beta1, beta2, eps, decay, rest1, rest2;       // rest = 1 - beta, rounded from 64 bits
     double ln1, ln2;                // ln(beta)
 };
 
-// A stretch [lo, hi) of tensor t, as chunk b of a table.  The lanes of a wave compare 64 entries at a time: two loads
-// deep, where a bisection through the kernel's arguments would be six or seven.
-struct Chunk {
-    int t;
-    bool first;         // of its tensor
-    int64_t lo, hi;
+// Elements between the start of a pointer's line of memory and the pointer.
+constexpr int kLine = 128;
+__host__ __device__ inline int shift_of(const void* p, int size) { return (int)((uintptr_t)p % kLine) / size; }
+
+// The workgroup's place in a table: chunk b as the stretch [lo, hi) of tensor t; lo is -shift in a tensor's first chunk.
+// A workgroup's next chunk is mostly one of the same tensor, for which nothing is looked up.  Otherwise the lanes of a
+// wave compare 64 entries at a time: two loads deep, where a bisection through the kernel's arguments would be six to eight.
+struct Cursor {
+    int t = 0, first = 0, end = 0;      // the tensor, its first chunk and the first one behind it
+    int shift = 0;
+    int64_t numel = 0, lo = 0, hi = 0;
+
+    // The tensor of chunk b (b ascends) -> whether it is another one than before.
+    template <int CAP>
+    __device__ __forceinline__ bool seek(const Chunks<CAP>& tab, int b) {
+        if (b < end) return false;
+        int before = 0;
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int base = 0; base < CAP; base += 64) {
+            const int i = base + lane;
+            before += __popcll(__ballot(i < tab.n && tab.end[i < tab.n ? i : 0] <= b));
+        }
+        t = __builtin_amdgcn_readfirstlane(before);
+        first = t ? tab.end[t - 1] : 0;
+        end = tab.end[t];
+        return true;
+    }
+    // `lead`: the pointer whose lines the chunks go by.
+    template <int CAP, typename T>
+    __device__ __forceinline__ void align(const Chunks<CAP>& tab, const T* lead) {
+        shift = shift_of(lead, sizeof(T));
+        numel = (int64_t)(end - first - 1) * tab.chunk + tab.tail[t] - shift;
+    }
+    template <int CAP>
+    __device__ __forceinline__ void range(const Chunks<CAP>& tab, int b) {
+        lo = (int64_t)(b - first) * tab.chunk - shift;
+        hi = lo + tab.chunk < numel ? lo + tab.chunk : numel;
+    }
 };
 
-template <typename Table, int CAP>
-__device__ __forceinline__ Chunk find_chunk(const Table& tab, const int (&end)[CAP], int b) {
-    int t = 0;
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int base = 0; base < CAP; base += 64) {
-        const int i = base + lane;
-        t += __popcll(__ballot(i < tab.n && end[i < tab.n ? i : 0] <= b));
-    }
-    t = __builtin_amdgcn_readfirstlane(t);
-    const int first = t ? end[t - 1] : 0;
-    Chunk c;
-    c.t = t;
-    c.first = b == first;
-    c.lo = (int64_t)(b - first) * tab.chunk;
-    c.hi = c.lo + tab.chunk < tab.numel[t] ? c.lo + tab.chunk : tab.numel[t];
-    return c;
-}
-
-// Sixteen bytes per lane and access.  A tensor may start at any multiple of its element size, so the type promises no
-// more than that; the hardware takes such addresses in one access all the same.
-template <typename T, int N>
+// One access of a lane.  The type promises no more alignment than an element's (the tensors of one parameter may lie at
+// different places of their 16 bytes); the hardware takes such addresses in one access all the same, if more slowly.
+// STREAM: past the caches, for lists that do not fit there.
+template <typename T, int N, bool STREAM>
 struct Pack {
     typedef T type __attribute__((ext_vector_type(N)));
     typedef type loose __attribute__((aligned(sizeof(T))));
-    static __device__ __forceinline__ type load(const T* p) { return *(const loose*)p; }
-    static __device__ __forceinline__ void store(T* p, type x) { *(loose*)p = x; }
+    static __device__ __forceinline__ type load(const T* p) {
+        return STREAM ? __builtin_nontemporal_load((const loose*)p) : *(const loose*)p;
+    }
+    static __device__ __forceinline__ void store(T* p, type x) {
+        if (STREAM) __builtin_nontemporal_store(x, (loose*)p);
+        else *(loose*)p = x;
+    }
 };
 
 // ---- sums in a fixed order --------------------------------------------------------------------------------------
@@ -123,6 +152,12 @@ template <int KIND>
 __device__ __forceinline__ double join(double a, double b) {
     if (KIND != NERF_NORM_MAX) return a + b;
     return __double_as_longlong(a) > __double_as_longlong(b) ? a : b;
+}
+
+template <int KIND>
+__device__ __forceinline__ double take(double acc, float x) {
+    if (KIND == NERF_NORM_L2) return fma((double)x, (double)x, acc);
+    return join<KIND>(acc, (double)fabsf(x));
 }
 
 template <int KIND>
@@ -157,22 +192,27 @@ __device__ __forceinline__ float coefficient(double norm, double max_norm) {
     return d <= max_norm ? 1.f : (float)(max_norm / d);       // (a NaN norm gives NaN)
 }
 
-template <int KIND>
-__device__ __forceinline__ double take(double acc, float x) {
-    if (KIND == NERF_NORM_L2) return fma((double)x, (double)x, acc);
-    return join<KIND>(acc, (double)fabsf(x));
-}
-
-template <typename T, int KIND>
-__global__ __launch_bounds__(kThreads) void norm_partials(NormTable tab, double* partials, float* steps) {
+template <typename T, int KIND, bool STREAM, typename Table>
+__global__ __launch_bounds__(kThreads) void norm_partials(Table tab, double* partials, float* steps) {
     constexpr int V = 16 / sizeof(T), kStep = kThreads * V, kDeep = 4;
-    using P = Pack<T, V>;
+    using P = Pack<T, V, STREAM>;
     double acc[2] = {0.0, 0.0};
     const int total = tab.end[tab.n - 1];
+    Cursor c;
+    const T* g = nullptr;
     for (int b = blockIdx.x; b < total; b += gridDim.x) {
-        const Chunk c = find_chunk(tab, tab.end, b);
-        const T* g = (const T*)tab.ptr[c.t];
+        if (c.seek(tab, b)) {
+            g = (const T*)tab.ptr[c.t];
+            c.align(tab, g);
+        }
+        if constexpr (std::is_same<Table, NormStepTable>::value)
+            if (b == c.first && threadIdx.x == 0) steps[tab.id[c.t]] = *tab.step[c.t];
+        c.range(tab, b);
         int64_t i = c.lo + threadIdx.x * V;
+        if (i < 0) {                                    // the first lanes of a tensor that starts inside a line
+            for (int64_t j = 0; j < i + V && j < c.hi; ++j) acc[0] = take<KIND>(acc[0], (float)g[j]);
+            i += kStep;
+        }
         for (; i + (kDeep - 1) * kStep + V <= c.hi; i += kDeep * kStep) {
             typename P::type x[kDeep];
 #pragma unroll
@@ -188,10 +228,9 @@ __global__ __launch_bounds__(kThreads) void norm_partials(NormTable tab, double*
             for (int j = 0; j < V; ++j) acc[j & 1] = take<KIND>(acc[j & 1], (float)x[j]);
         }
         for (; i < c.hi; ++i) acc[0] = take<KIND>(acc[0], (float)g[i]);     // the last lane's rest
-        if (c.first && threadIdx.x == 0 && tab.step[c.t]) steps[tab.id[c.t]] = *tab.step[c.t];
     }
     const double sum = group_join<KIND>(join<KIND>(acc[0], acc[1]));
-    if (threadIdx.x == 0) partials[tab.first_partial + blockIdx.x] = sum;
+    if (threadIdx.x == 0) partials[blockIdx.x] = sum;
 }
 
 __global__ __launch_bounds__(kThreads) void norm_finish(Clip clip) {
@@ -204,32 +243,34 @@ __global__ __launch_bounds__(kThreads) void read_steps(StepTable tab, float* ste
     if (i < tab.n) steps[tab.first_tensor + i] = *tab.step[i];
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void scale_by_norm(ScaleTable tab, Clip clip) {
+template <typename T, bool STREAM>
+__global__ __launch_bounds__(kThreads) void scale_by_norm(ListTable tab, Clip clip) {
     constexpr int V = 16 / sizeof(T), kStep = kThreads * V;
-    using P = Pack<T, V>;
+    using P = Pack<T, V, STREAM>;
     const double norm = norm_of(clip);
     if (blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = (float)norm;
     const float s = coefficient(norm, clip.max_norm);
     const int total = tab.end[tab.n - 1];
+    Cursor c;
+    T* g = nullptr;
     for (int b = blockIdx.x; b < total; b += gridDim.x) {
-        const Chunk c = find_chunk(tab, tab.end, b);
-        T* g = (T*)tab.ptr[c.t];
-        int64_t i = c.lo + threadIdx.x * V;
-        for (; i + V <= c.hi; i += kStep) {
-            typename P::type x = P::load(g + i);
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = (T)((float)x[j] * s);
-            P::store(g + i, x);
+        if (c.seek(tab, b)) {
+            g = (T*)tab.ptr[c.t];
+            c.align(tab, g);
         }
-        for (; i < c.hi; ++i) g[i] = (T)((float)g[i] * s);
+        c.range(tab, b);
+        for (int64_t i = c.lo + threadIdx.x * V; i < c.hi; i += kStep) {
+            if (i >= 0 && i + V <= c.hi) {
+                typename P::type x = P::load(g + i);
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[j] = (T)((float)x[j] * s);
+                P::store(g + i, x);
+            } else {
+                for (int64_t j = i < 0 ? 0 : i; j < i + V && j < c.hi; ++j) g[j] = (T)((float)g[j] * s);
+            }
+        }
     }
 }
-
-// A 16-bit parameter is the rounding of its 32-bit master.  Left to itself the compiler forms the last multiply-add
-// and the conversion to fp16 as one instruction, which rounds the exact sum once and so may end on the other neighbour
-// than the rounding of the rounded sum: the value has to exist in 32 bits first.
-__device__ __forceinline__ void keep_rounded(float& x) { asm("" : "+v"(x)); }
 
 struct Factors {
     float clip, lr, inv1, inv2;     // inv1 = 1 / (1 - beta1^t), inv2 = 1 / sqrt(1 - beta2^t)
@@ -250,12 +291,17 @@ __device__ __forceinline__ float weight_of(T p, float master) {
     return (T)master == p ? master : (float)p;
 }
 
-template <typename T>
+// A 16-bit parameter is the rounding of its 32-bit master.  Left to itself the compiler forms the last multiply-add
+// and the conversion to fp16 as one instruction, which rounds the exact sum once and so may end on the other neighbour
+// than the rounding of the rounded sum: the value has to exist in 32 bits first.
+__device__ __forceinline__ void keep_rounded(float& x) { asm("" : "+v"(x)); }
+
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(kThreads) void adamw(AdamTable tab, Clip clip, AdamArgs a, const float* steps) {
     constexpr bool kMaster = sizeof(T) == 2;
     constexpr int V = 4, kStep = kThreads * V;
-    using P = Pack<T, V>;
-    using F = Pack<float, V>;
+    using P = Pack<T, V, STREAM>;
+    using F = Pack<float, V, STREAM>;
     Factors f;
     f.clip = 1.f;
     if (clip.partials) {
@@ -266,39 +312,48 @@ __global__ __launch_bounds__(kThreads) void adamw(AdamTable tab, Clip clip, Adam
     }
     f.lr = a.lr_ptr ? *a.lr_ptr : a.lr;
     const int total = tab.end[tab.n - 1];
+    Cursor c;
+    T* p = nullptr;
+    const T* g = nullptr;
+    float *m = nullptr, *v = nullptr, *w = nullptr;
     for (int b = blockIdx.x; b < total; b += gridDim.x) {
-        const Chunk c = find_chunk(tab, tab.end, b);
-        const float now = steps[tab.id[c.t]] + 1.f;
-        if (c.first && threadIdx.x == 0) *tab.step[c.t] = now;
-        f.inv1 = 1.f / -expm1f((float)(now * a.ln1));
-        f.inv2 = 1.f / sqrtf(-expm1f((float)(now * a.ln2)));
-        T* p = (T*)tab.p[c.t];
-        const T* g = (const T*)tab.g[c.t];
-        float *m = tab.m[c.t], *v = tab.v[c.t], *w = tab.w[c.t];
-        int64_t i = c.lo + threadIdx.x * V;
-        for (; i + V <= c.hi; i += kStep) {
-            typename P::type pi = P::load(p + i);
-            const typename P::type gi = P::load(g + i);
-            typename F::type mi = F::load(m + i), vi = F::load(v + i), wi = {};
-            if (kMaster) wi = F::load(w + i);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float wj = kMaster ? weight_of<T>(pi[j], wi[j]) : (float)pi[j], mj = mi[j], vj = vi[j];
-                adamw_entry(wj, (float)gi[j], mj, vj, a, f);
-                if (kMaster) keep_rounded(wj);
-                wi[j] = wj, mi[j] = mj, vi[j] = vj, pi[j] = (T)wj;
-            }
-            P::store(p + i, pi);
-            F::store(m + i, mi);
-            F::store(v + i, vi);
-            if (kMaster) F::store(w + i, wi);
+        if (c.seek(tab, b)) {
+            const float now = steps[tab.id[c.t]] + 1.f;
+            if (b == c.first && threadIdx.x == 0) *tab.step[c.t] = now;
+            f.inv1 = 1.f / -expm1f((float)(now * a.ln1));
+            f.inv2 = 1.f / sqrtf(-expm1f((float)(now * a.ln2)));
+            p = (T*)tab.p[c.t];
+            g = (const T*)tab.g[c.t];
+            m = tab.m[c.t], v = tab.v[c.t], w = tab.w[c.t];
+            c.align(tab, m);
         }
-        for (; i < c.hi; ++i) {
-            float wi = kMaster ? weight_of<T>(p[i], w[i]) : (float)p[i], mi = m[i], vi = v[i];
-            adamw_entry(wi, (float)g[i], mi, vi, a, f);
-            if (kMaster) keep_rounded(wi);
-            m[i] = mi, v[i] = vi, p[i] = (T)wi;
-            if (kMaster) w[i] = wi;
+        c.range(tab, b);
+        for (int64_t i = c.lo + threadIdx.x * V; i < c.hi; i += kStep) {
+            if (i >= 0 && i + V <= c.hi) {
+                typename P::type pi = P::load(p + i);
+                const typename P::type gi = P::load(g + i);
+                typename F::type mi = F::load(m + i), vi = F::load(v + i), wi = {};
+                if (kMaster) wi = F::load(w + i);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float wj = kMaster ? weight_of<T>(pi[j], wi[j]) : (float)pi[j], mj = mi[j], vj = vi[j];
+                    adamw_entry(wj, (float)gi[j], mj, vj, a, f);
+                    if (kMaster) keep_rounded(wj);
+                    wi[j] = wj, mi[j] = mj, vi[j] = vj, pi[j] = (T)wj;
+                }
+                P::store(p + i, pi);
+                F::store(m + i, mi);
+                F::store(v + i, vi);
+                if (kMaster) F::store(w + i, wi);
+            } else {
+                for (int64_t j = i < 0 ? 0 : i; j < i + V && j < c.hi; ++j) {
+                    float wj = kMaster ? weight_of<T>(p[j], w[j]) : (float)p[j], mj = m[j], vj = v[j];
+                    adamw_entry(wj, (float)g[j], mj, vj, a, f);
+                    if (kMaster) keep_rounded(wj);
+                    m[j] = mj, v[j] = vj, p[j] = (T)wj;
+                    if (kMaster) w[j] = wj;
+                }
+            }
         }
     }
 }
@@ -307,7 +362,7 @@ __global__ __launch_bounds__(kThreads) void adamw(AdamTable tab, Clip clip, Adam
 
 bool known_dtype(int d) { return d == NERF_F32 || d == NERF_BF16 || d == NERF_F16; }
 bool known_kind(int k) { return k == NERF_NORM_L1 || k == NERF_NORM_L2 || k == NERF_NORM_MAX; }
-int64_t elem_size(int d) { return d == NERF_F32 ? 4 : 2; }
+int elem_size(int d) { return d == NERF_F32 ? 4 : 2; }
 
 int check_list(const void* const* ptr, const int64_t* numel, const int32_t* dtype, int n) {
     NERF_REQUIRE(n >= 0);
@@ -348,24 +403,29 @@ int check_disjoint(void* const* ptr, const int64_t* numel, const int32_t* dtype,
     return apart ? NERF_OK : NERF_ERR_ARG;
 }
 
-// Elements per chunk: as few as kMinChunk while the list is short (latency: every compute unit gets some), up to
-// kMaxChunk for a long one (a chunk's lookup is paid once per kMaxChunk elements), more only where 2^30 chunks would not
-// do.
-int chunk_for(const int64_t* numel, int n) {
-    int64_t total = 0;
-    for (int i = 0; i < n; ++i) total += numel[i];
-    int64_t chunk = kMinChunk;
-    while ((chunk < kMaxChunk && total / chunk > kMaxGroups) || total / chunk > ((int64_t)1 << 30)) chunk *= 2;
+// ---- launches ---------------------------------------------------------------------------------------------------
+
+// Elements per chunk of a list of `total`; beyond 2^30 chunks they get longer than `most`.
+int chunk_for(int64_t total, const Cut& cut) {
+    int64_t chunk = cut.least;
+    while ((chunk < cut.most && total / chunk > cut.groups) || total / chunk > ((int64_t)1 << 30)) chunk *= 2;
     return (int)chunk;
 }
 
-int groups_for(int chunks) { return chunks < kMaxGroups ? chunks : kMaxGroups; }
+int64_t list_elements(const int64_t* numel, int n) {
+    int64_t total = 0;
+    for (int i = 0; i < n; ++i) total += numel[i];
+    return total;
+}
 
-// a tensor without elements has one empty chunk (its step counter still counts)
-int chunks_of(int64_t numel, int chunk) { return numel ? (int)((numel + chunk - 1) / chunk) : 1; }
+int64_t list_bytes(const int64_t* numel, const int32_t* dtype, int n) {
+    int64_t total = 0;
+    for (int i = 0; i < n; ++i) total += numel[i] * elem_size(dtype[i]);
+    return total;
+}
 
-// A launch leaves at most kMaxGroups partials, and there are as many launches as full tables and one more per type.
-int64_t max_partials(int n) { return (int64_t)kMaxGroups * (3 + n / kNormCap); }
+// A launch leaves at most kNormGroups partials, and there are as many launches as full tables and one more per type.
+int64_t max_partials(int n) { return (int64_t)kNormGroups * (3 + n / NormStepTable::kCap); }
 
 struct Workspace {
     double* partials;
@@ -381,56 +441,72 @@ int take_workspace(void* ws, int64_t bytes, int n, Workspace* out) {
     return NERF_OK;
 }
 
-constexpr int kDtypes[] = {NERF_F32, NERF_BF16, NERF_F16};
-
-// fill(k, i) puts tensor i into place k of a table; go(d) launches a full one, and the last of each type.
-template <typename Table, int CAP, typename Fill, typename Go>
-void for_tables(Table& tab, int (&ends)[CAP], const int64_t* numel, const int32_t* dtype, int first, int last, Fill fill, Go go) {
-    for (int d : kDtypes) {
+// Tensors first .. last - 1 of a list of `total` elements, type by type: shift(i, element size) is shift_of its
+// leading pointer; fill(k, i) puts it into place k of a table; go(type, workgroups) launches a full table, and the last of each
+// type.  A tensor without elements has one empty chunk (its step counter still counts).
+template <typename Table, typename Shift, typename Fill, typename Go>
+void for_tables(Table& tab, Cut (*cut_of)(int), int64_t total, const int64_t* numel, const int32_t* dtype, int first, int last,
+                Shift shift, Fill fill, Go go) {
+    for (int d : {NERF_F32, NERF_BF16, NERF_F16}) {
+        const Cut cut = cut_of(elem_size(d));
+        tab.chunk = chunk_for(total, cut);
         tab.n = 0;
         int end = 0;
         for (int i = first; i < last; ++i) {
             if (dtype[i] != d) continue;
-            end += chunks_of(numel[i], tab.chunk);
+            const int64_t span = numel[i] + shift(i, elem_size(d));
+            const int chunks = std::max(1, (int)((span + tab.chunk - 1) / tab.chunk));
+            end += chunks;
             fill(tab.n, i);
-            tab.numel[tab.n] = numel[i];
-            ends[tab.n] = end;
-            if (++tab.n == CAP) {
-                go(d, groups_for(end));
+            tab.end[tab.n] = end;
+            tab.tail[tab.n] = (int)(span - (int64_t)(chunks - 1) * tab.chunk);
+            if (++tab.n == Table::kCap) {
+                go(d, std::min(end, cut.groups));
                 tab.n = end = 0;
             }
         }
-        if (tab.n) go(d, groups_for(end));
+        if (tab.n) go(d, std::min(end, cut.groups));
     }
 }
 
-template <typename T>
-void launch_norm(const NormTable& tab, int grid, int kind, const Workspace& ws, hipStream_t st) {
-    if (kind == NERF_NORM_L2) norm_partials<T, NERF_NORM_L2><<<grid, kThreads, 0, st>>>(tab, ws.partials, ws.steps);
-    else if (kind == NERF_NORM_L1) norm_partials<T, NERF_NORM_L1><<<grid, kThreads, 0, st>>>(tab, ws.partials, ws.steps);
-    else norm_partials<T, NERF_NORM_MAX><<<grid, kThreads, 0, st>>>(tab, ws.partials, ws.steps);
+// go(element, streams) with values that carry the types of a kernel's instantiation.
+template <typename Go>
+void by_type(int d, bool streams, Go go) {
+    const std::true_type yes;
+    const std::false_type no;
+    if (d == NERF_F32) streams ? go(float(), yes) : go(float(), no);
+    else if (d == NERF_BF16) streams ? go(__bf16(), yes) : go(__bf16(), no);
+    else streams ? go(_Float16(), yes) : go(_Float16(), no);
 }
 
-// The norm's first launch(es): a partial per workgroup.
-int run_norm(const void* const* ptr, float* const* step, const int64_t* numel, const int32_t* dtype, int n, int kind,
-             const Workspace& ws, int* n_partials, hipStream_t st) {
-    NormTable tab;
-    tab.chunk = chunk_for(numel, n);
-    tab.first_partial = 0;
-    for_tables(tab, tab.end, numel, dtype, 0, n,
+template <typename T, bool STREAM, typename Table>
+void launch_norm(const Table& tab, int grid, int kind, double* partials, float* steps, hipStream_t st) {
+    if (kind == NERF_NORM_L2) norm_partials<T, NERF_NORM_L2, STREAM><<<grid, kThreads, 0, st>>>(tab, partials, steps);
+    else if (kind == NERF_NORM_L1) norm_partials<T, NERF_NORM_L1, STREAM><<<grid, kThreads, 0, st>>>(tab, partials, steps);
+    else norm_partials<T, NERF_NORM_MAX, STREAM><<<grid, kThreads, 0, st>>>(tab, partials, steps);
+}
+
+// The norm's launches ahead of its reader's: a partial per workgroup -> how many.  more(k, i) fills what else the table
+// holds.
+template <bool CAN_STREAM, typename Table, typename More>
+int run_norm(Table& tab, const void* const* ptr, const int64_t* numel, const int32_t* dtype, int n, int kind,
+             const Workspace& ws, hipStream_t st, More more) {
+    int partials = 0;
+    const bool streams = CAN_STREAM && list_bytes(numel, dtype, n) > kNormStream;
+    for_tables(tab, norm_cut, list_elements(numel, n), numel, dtype, 0, n,
+               [&](int i, int size) { return shift_of(ptr[i], size); },
                [&](int k, int i) {
-                   tab.ptr[k] = ptr[i];
-                   tab.step[k] = step ? step[i] : nullptr;
-                   tab.id[k] = i;
+                   tab.ptr[k] = const_cast<void*>(ptr[i]);
+                   more(k, i);
                },
                [&](int d, int grid) {
-                   if (d == NERF_F32) launch_norm<float>(tab, grid, kind, ws, st);
-                   else if (d == NERF_BF16) launch_norm<__bf16>(tab, grid, kind, ws, st);
-                   else launch_norm<_Float16>(tab, grid, kind, ws, st);
-                   tab.first_partial += grid;
+                   by_type(d, streams, [&](auto element, auto stream) {
+                       launch_norm<decltype(element), CAN_STREAM && decltype(stream)::value>(
+                           tab, grid, kind, ws.partials + partials, ws.steps, st);
+                   });
+                   partials += grid;
                });
-    *n_partials = tab.first_partial;
-    return nerf_launch_status();
+    return partials;
 }
 
 }  // namespace
@@ -438,46 +514,47 @@ int run_norm(const void* const* ptr, float* const* step, const int64_t* numel, c
 extern "C" int64_t nerf_grad_workspace_bytes(int n_tensors) { return n_tensors < 0 ? NERF_ERR_ARG : workspace_bytes(n_tensors); }
 
 extern "C" int nerf_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtype, int n_tensors,
-                              int norm_kind, void* workspace, int64_t workspace_bytes_, float* norm, void* stream) {
+                              int norm_kind, void* workspace, int64_t n_workspace, float* norm, void* stream) {
     if (int e = check_list(grads, numel, dtype, n_tensors)) return e;
     NERF_REQUIRE(known_kind(norm_kind) && norm);
     Workspace ws;
-    if (int e = take_workspace(workspace, workspace_bytes_, n_tensors, &ws)) return e;
-    int partials = 0;
-    if (int e = run_norm(grads, nullptr, numel, dtype, n_tensors, norm_kind, ws, &partials, nerf_stream(stream))) return e;
-    norm_finish<<<1, kThreads, 0, nerf_stream(stream)>>>(Clip{ws.partials, partials, norm_kind, 0, 0.0, norm});
+    if (int e = take_workspace(workspace, n_workspace, n_tensors, &ws)) return e;
+    hipStream_t st = nerf_stream(stream);
+    ListTable tab;
+    const int partials = run_norm<true>(tab, grads, numel, dtype, n_tensors, norm_kind, ws, st, [](int, int) {});
+    norm_finish<<<1, kThreads, 0, st>>>(Clip{ws.partials, partials, norm_kind, 0, 0.0, norm});
     return nerf_launch_status();
 }
 
 extern "C" int nerf_clip_grad_norm(void* const* grads, const int64_t* numel, const int32_t* dtype, int n_tensors,
-                                   int norm_kind, double max_norm, void* workspace, int64_t workspace_bytes_, float* norm,
+                                   int norm_kind, double max_norm, void* workspace, int64_t n_workspace, float* norm,
                                    void* stream) {
     if (int e = check_list(grads, numel, dtype, n_tensors)) return e;
     NERF_REQUIRE(known_kind(norm_kind) && max_norm >= 0.0 && norm);
     Workspace ws;
-    if (int e = take_workspace(workspace, workspace_bytes_, n_tensors, &ws)) return e;
+    if (int e = take_workspace(workspace, n_workspace, n_tensors, &ws)) return e;
     if (int e = check_disjoint(grads, numel, dtype, n_tensors)) return e;
     hipStream_t st = nerf_stream(stream);
-    int partials = 0;
-    if (int e = run_norm(grads, nullptr, numel, dtype, n_tensors, norm_kind, ws, &partials, st)) return e;
+    ListTable tab;
+    const int partials = run_norm<false>(tab, grads, numel, dtype, n_tensors, norm_kind, ws, st, [](int, int) {});
     const Clip clip{ws.partials, partials, norm_kind, 0, max_norm, norm};
     if (n_tensors == 0) {
         norm_finish<<<1, kThreads, 0, st>>>(clip);
         return nerf_launch_status();
     }
-    ScaleTable tab;
-    tab.chunk = chunk_for(numel, n_tensors);
-    for_tables(tab, tab.end, numel, dtype, 0, n_tensors, [&](int k, int i) { tab.ptr[k] = grads[i]; },
+    const bool streams = 2 * list_bytes(numel, dtype, n_tensors) > kUpdateStream;
+    for_tables(tab, scale_cut, list_elements(numel, n_tensors), numel, dtype, 0, n_tensors,
+               [&](int i, int size) { return shift_of(grads[i], size); }, [&](int k, int i) { tab.ptr[k] = grads[i]; },
                [&](int d, int grid) {
-                   if (d == NERF_F32) scale_by_norm<float><<<grid, kThreads, 0, st>>>(tab, clip);
-                   else if (d == NERF_BF16) scale_by_norm<__bf16><<<grid, kThreads, 0, st>>>(tab, clip);
-                   else scale_by_norm<_Float16><<<grid, kThreads, 0, st>>>(tab, clip);
+                   by_type(d, streams, [&](auto element, auto s) {
+                       scale_by_norm<decltype(element), decltype(s)::value><<<grid, kThreads, 0, st>>>(tab, clip);
+                   });
                });
     return nerf_launch_status();
 }
 
 extern "C" int nerf_adamw_step(const nerf_adamw_tensors* t, const nerf_adamw_group* groups, int n_groups, int norm_kind,
-                               double max_norm, int skip_nonfinite, void* workspace, int64_t workspace_bytes_, float* norm,
+                               double max_norm, int skip_nonfinite, void* workspace, int64_t n_workspace, float* norm,
                                void* stream) {
     NERF_REQUIRE(t && n_groups >= 0 && (groups || n_groups == 0));
     const int n = t->n_tensors;
@@ -506,7 +583,7 @@ extern "C" int nerf_adamw_step(const nerf_adamw_tensors* t, const nerf_adamw_gro
     NERF_REQUIRE(clips || !skip_nonfinite);
     if (n == 0) return NERF_OK;
     Workspace ws;
-    if (int e = take_workspace(workspace, workspace_bytes_, n, &ws)) return e;
+    if (int e = take_workspace(workspace, n_workspace, n, &ws)) return e;
     if (int e = check_disjoint(t->param, t->numel, t->dtype, n)) return e;
     hipStream_t st = nerf_stream(stream);
     Clip clip{nullptr, 0, norm_kind, skip_nonfinite, max_norm, norm};
@@ -514,7 +591,11 @@ extern "C" int nerf_adamw_step(const nerf_adamw_tensors* t, const nerf_adamw_gro
     // update the first workgroup of a tensor writes a counter that the others of that tensor need the old value of.
     if (clips) {
         clip.partials = ws.partials;
-        if (int e = run_norm(t->grad, t->step, t->numel, t->dtype, n, norm_kind, ws, &clip.n_partials, st)) return e;
+        NormStepTable norms;
+        clip.n_partials = run_norm<false>(norms, t->grad, t->numel, t->dtype, n, norm_kind, ws, st, [&](int k, int i) {
+            norms.step[k] = t->step[i];
+            norms.id[k] = i;
+        });
     } else {
         StepTable s;
         for (s.first_tensor = 0; s.first_tensor < n; s.first_tensor += s.n) {
@@ -522,14 +603,16 @@ extern "C" int nerf_adamw_step(const nerf_adamw_tensors* t, const nerf_adamw_gro
             read_steps<<<1, kThreads, 0, st>>>(s, ws.steps);
         }
     }
+    const int64_t elements = list_elements(t->numel, n);
+    const bool streams = 28 * elements > kUpdateStream;
     AdamTable tab;
-    tab.chunk = chunk_for(t->numel, n);
     int first = 0;
     for (int k = 0; k < n_groups; ++k) {
         const nerf_adamw_group& g = groups[k];
-        const AdamArgs a{g.lr_device, (float)g.lr, (float)g.beta2, (float)g.eps, (float)g.weight_decay, (float)(1.0 - g.beta1),
-                         (float)(1.0 - g.beta2), (float)g.beta1, log(g.beta1), log(g.beta2)};
-        for_tables(tab, tab.end, t->numel, t->dtype, first, first + g.count,
+        const AdamArgs a{g.lr_device,          (float)g.lr,           (float)g.beta1, (float)g.beta2, (float)g.eps,
+                         (float)g.weight_decay, (float)(1.0 - g.beta1), (float)(1.0 - g.beta2), log(g.beta1), log(g.beta2)};
+        for_tables(tab, adam_cut, elements, t->numel, t->dtype, first, first + g.count,
+                   [&](int i, int) { return shift_of(t->exp_avg[i], 4); },
                    [&](int j, int i) {
                        tab.p[j] = t->param[i];
                        tab.g[j] = t->grad[i];
@@ -540,9 +623,9 @@ extern "C" int nerf_adamw_step(const nerf_adamw_tensors* t, const nerf_adamw_gro
                        tab.id[j] = i;
                    },
                    [&](int d, int grid) {
-                       if (d == NERF_F32) adamw<float><<<grid, kThreads, 0, st>>>(tab, clip, a, ws.steps);
-                       else if (d == NERF_BF16) adamw<__bf16><<<grid, kThreads, 0, st>>>(tab, clip, a, ws.steps);
-                       else adamw<_Float16><<<grid, kThreads, 0, st>>>(tab, clip, a, ws.steps);
+                       by_type(d, streams, [&](auto element, auto s) {
+                           adamw<decltype(element), decltype(s)::value><<<grid, kThreads, 0, st>>>(tab, clip, a, ws.steps);
+                       });
                    });
         first += g.count;
     }
