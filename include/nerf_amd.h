@@ -170,7 +170,7 @@ int nerf_scatter_fwd(const float* rgb, const float* angle, const float* density,
  * call on a GPU uses that GPU's one array: calls that overlap on one GPU (two streams, two threads) race.
  * The first call on each device looks the array's address up (hipGetSymbolAddress: a module lookup, not a stream
  * operation); make that one call outside any stream capture, on every device that will capture -- later calls only
- * enqueue two memsets and two kernels and may be captured (tests/test_zz_no_alloc.py replays such a graph). */
+ * enqueue three kernels and may be captured (tests/test_zz_no_alloc.py replays such a graph). */
 int nerf_scatter_fwd_static(const float* rgb, const float* angle, const float* density, const float* power,
                             const float* t_vals, const float* dirs, const float* pulse_bins, int64_t n_rays,
                             int num_samples, int nsam, float wavelength, const nerf_activation* act,

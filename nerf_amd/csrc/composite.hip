@@ -299,6 +299,15 @@ __global__ void scatter_fwd_kernel(const float* __restrict__ rgb, const float* _
     }
 }
 
+// Ahead of the scatter: no ray has won any bin, no ray is out of range.  A kernel and not a memset: memset nodes of a
+// captured graph have left the buffer as it was on replays after the first, and what another tensor had put there since
+// was then taken for ray indices by the kernel below.
+__global__ void scatter_clear_kernel(int32_t* __restrict__ winner, int nsam, int32_t* __restrict__ status) {
+    const int b = blockIdx.x * blockDim.x + threadIdx.x;
+    if (b < nsam) winner[b] = -1;
+    if (b == 0) *status = 0;
+}
+
 __global__ void scatter_write_kernel(const float* __restrict__ ray_ret, const int32_t* __restrict__ winner, int nsam,
                                      float* __restrict__ pulse) {
     const int b = blockIdx.x * blockDim.x + threadIdx.x;
@@ -411,8 +420,7 @@ extern "C" int nerf_scatter_fwd(const float* rgb, const float* angle, const floa
                  ray_ret && ray_bin && comp && winner && status);
     NERF_REQUIRE(n_rays >= 0 && num_samples >= 1 && nsam >= 1 && wavelength > 0.f);
     hipStream_t st = nerf_stream(stream);
-    if (hipMemsetAsync(winner, 0xFF, (size_t)nsam * sizeof(int32_t), st) != hipSuccess) return NERF_ERR_LAUNCH;
-    if (hipMemsetAsync(status, 0, sizeof(int32_t), st) != hipSuccess) return NERF_ERR_LAUNCH;
+    hipLaunchKernelGGL(scatter_clear_kernel, dim3(nerf_blocks(nsam, 256)), dim3(256), 0, st, winner, nsam, status);
     if (n_rays > 0) {
         hipLaunchKernelGGL(scatter_fwd_kernel, dim3(nerf_blocks(n_rays, kWavesPerBlock)), dim3(64 * kWavesPerBlock),
                            0, st, rgb, angle, density, power, t_vals, dirs, pulse_bins, n_rays, num_samples, nsam,
@@ -430,7 +438,7 @@ extern "C" int nerf_scatter_fwd(const float* rgb, const float* angle, const floa
 // the scatter -- the per-bin winner indices and the per-ray complex returns -- live in a file-scope device array
 // instead of coming from the caller.  Each GPU holds its own copy of the array at its own address; that address
 // is looked up once per device, on the first call made with that device current, and only it (never the array's
-// name, which in host code is a stand-in and not a device address) is handed to memsets and kernels.
+// name, which in host code is a stand-in and not a device address) is handed to kernels.
 constexpr int kStaticMaxBins = 65536;       // nsam     <= 65536: 256 KiB of winners
 constexpr int kStaticMaxRays = 65536;       // n_rays   <= 65536: 512 KiB of returns
 static __device__ __align__(256) unsigned char scratch[(size_t)kStaticMaxBins * 4 + (size_t)kStaticMaxRays * 8];
