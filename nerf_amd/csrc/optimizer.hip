@@ -32,7 +32,7 @@ struct Cut {
 constexpr int kNormGroups = 1024;
 constexpr Cut norm_cut(int size) { return {kNormGroups, 4096 / size, 32768 / size}; }
 constexpr Cut scale_cut(int size) { return {1024, 4096 / size, 16384 / size}; }
-constexpr Cut adam_cut(int) { return {768, 1024, 4096}; }
+constexpr Cut adam_cut(int) { return {768, 1024, 2048}; }
 
 constexpr int64_t kMiB = 1 << 20;
 constexpr int64_t kNormStream = 64 * kMiB;
@@ -92,36 +92,37 @@ constexpr int kLine = 128;
 __host__ __device__ inline int shift_of(const void* p, int size) { return (int)((uintptr_t)p % kLine) / size; }
 
 // The workgroup's place in a table: chunk b as the stretch [lo, hi) of tensor t; lo is -shift in a tensor's first chunk.
-// A workgroup's next chunk is mostly one of the same tensor, for which nothing is looked up.  Otherwise the lanes of a
-// wave compare 64 entries at a time: two loads deep, where a bisection through the kernel's arguments would be six to eight.
+// Among tensors of under a thousand chunks a workgroup's next chunk is mostly another tensor's, so that lookups are on
+// the path of every chunk: the lanes of each wave hold the table's `end` in registers and compare all of it at once.
+template <int CAP>
 struct Cursor {
+    static constexpr int kRegs = (CAP + 63) / 64;
+    int ends[kRegs];
     int t = 0, first = 0, end = 0;      // the tensor, its first chunk and the first one behind it
     int shift = 0;
     int64_t numel = 0, lo = 0, hi = 0;
 
-    // The tensor of chunk b (b ascends) -> whether it is another one than before.
-    template <int CAP>
-    __device__ __forceinline__ bool seek(const Chunks<CAP>& tab, int b) {
-        if (b < end) return false;
-        int before = 0;
+    __device__ __forceinline__ explicit Cursor(const Chunks<CAP>& tab) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int base = 0; base < CAP; base += 64) {
-            const int i = base + lane;
-            before += __popcll(__ballot(i < tab.n && tab.end[i < tab.n ? i : 0] <= b));
-        }
-        t = __builtin_amdgcn_readfirstlane(before);
+        for (int k = 0; k < kRegs; ++k) ends[k] = 64 * k + lane < tab.n ? tab.end[64 * k + lane] : 0x7fffffff;
+    }
+    // The tensor of chunk b (b ascends) -> whether it is another one than before.
+    __device__ __forceinline__ bool seek(const Chunks<CAP>& tab, int b) {
+        if (b < end) return false;
+        t = 0;
+#pragma unroll
+        for (int k = 0; k < kRegs; ++k) t += __popcll(__ballot(ends[k] <= b));
         first = t ? tab.end[t - 1] : 0;
         end = tab.end[t];
         return true;
     }
     // `lead`: the pointer whose lines the chunks go by.
-    template <int CAP, typename T>
+    template <typename T>
     __device__ __forceinline__ void align(const Chunks<CAP>& tab, const T* lead) {
         shift = shift_of(lead, sizeof(T));
         numel = (int64_t)(end - first - 1) * tab.chunk + tab.tail[t] - shift;
     }
-    template <int CAP>
     __device__ __forceinline__ void range(const Chunks<CAP>& tab, int b) {
         lo = (int64_t)(b - first) * tab.chunk - shift;
         hi = lo + tab.chunk < numel ? lo + tab.chunk : numel;
@@ -175,8 +176,15 @@ __device__ __forceinline__ double group_join(double x) {
 
 template <int KIND>
 __device__ __forceinline__ double norm_of(const double* partials, int n) {
+    constexpr int kDeep = 8;        // loads under way at once: every workgroup of the update waits for these
     double x = 0.0;
-    for (int i = threadIdx.x; i < n; i += kThreads) x = join<KIND>(x, partials[i]);
+    for (int i = threadIdx.x; i < n; i += kDeep * kThreads) {
+        double y[kDeep];
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k) y[k] = i + k * kThreads < n ? partials[i + k * kThreads] : 0.0;
+#pragma unroll
+        for (int k = 0; k < kDeep; ++k) x = join<KIND>(x, y[k]);
+    }
     x = group_join<KIND>(x);
     return KIND == NERF_NORM_L2 ? sqrt(x) : x;
 }
@@ -198,7 +206,7 @@ __global__ __launch_bounds__(kThreads) void norm_partials(Table tab, double* par
     using P = Pack<T, V, STREAM>;
     double acc[2] = {0.0, 0.0};
     const int total = tab.end[tab.n - 1];
-    Cursor c;
+    Cursor<Table::kCap> c(tab);
     const T* g = nullptr;
     for (int b = blockIdx.x; b < total; b += gridDim.x) {
         if (c.seek(tab, b)) {
@@ -251,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void scale_by_norm(ListTable tab, Clip cl
     if (blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = (float)norm;
     const float s = coefficient(norm, clip.max_norm);
     const int total = tab.end[tab.n - 1];
-    Cursor c;
+    Cursor<ListTable::kCap> c(tab);
     T* g = nullptr;
     for (int b = blockIdx.x; b < total; b += gridDim.x) {
         if (c.seek(tab, b)) {
@@ -270,6 +278,10 @@ __global__ __launch_bounds__(kThreads) void scale_by_norm(ListTable tab, Clip cl
             }
         }
     }
+}
+
+__device__ __forceinline__ float of_lane(float x, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
 struct Factors {
@@ -311,17 +323,21 @@ __global__ __launch_bounds__(kThreads) void adamw(AdamTable tab, Clip clip, Adam
         f.clip = coefficient(norm, clip.max_norm);
     }
     f.lr = a.lr_ptr ? *a.lr_ptr : a.lr;
+    // lane i of each wave computes the factors of tensor i, ahead of the first chunk
+    static_assert(AdamTable::kCap <= 64, "a lane per tensor");
+    const int lane = threadIdx.x & 63;
+    const float now = lane < tab.n ? steps[tab.id[lane]] + 1.f : 1.f;
+    const float inv1 = 1.f / -expm1f((float)(now * a.ln1)), inv2 = 1.f / sqrtf(-expm1f((float)(now * a.ln2)));
     const int total = tab.end[tab.n - 1];
-    Cursor c;
+    Cursor<AdamTable::kCap> c(tab);
     T* p = nullptr;
     const T* g = nullptr;
     float *m = nullptr, *v = nullptr, *w = nullptr;
     for (int b = blockIdx.x; b < total; b += gridDim.x) {
         if (c.seek(tab, b)) {
-            const float now = steps[tab.id[c.t]] + 1.f;
-            if (b == c.first && threadIdx.x == 0) *tab.step[c.t] = now;
-            f.inv1 = 1.f / -expm1f((float)(now * a.ln1));
-            f.inv2 = 1.f / sqrtf(-expm1f((float)(now * a.ln2)));
+            f.inv1 = of_lane(inv1, c.t);
+            f.inv2 = of_lane(inv2, c.t);
+            if (b == c.first && threadIdx.x == 0) *tab.step[c.t] = of_lane(now, c.t);
             p = (T*)tab.p[c.t];
             g = (const T*)tab.g[c.t];
             m = tab.m[c.t], v = tab.v[c.t], w = tab.w[c.t];

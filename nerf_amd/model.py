@@ -71,7 +71,12 @@ class _RenderModule(nn.Module):
 
     def configure_optimizers(self):
         cfg = self.config
-        optimizer = optim.AdamW(self.parameters(), lr=cfg.lr_init, weight_decay=cfg.weight_decay)
+        if getattr(cfg, 'fused_adamw', False):
+            from .optim import AdamW
+            optimizer = AdamW(self.parameters(), lr=cfg.lr_init, weight_decay=cfg.weight_decay,
+                              max_norm=getattr(cfg, 'max_grad_norm', None))
+        else:
+            optimizer = optim.AdamW(self.parameters(), lr=cfg.lr_init, weight_decay=cfg.weight_decay)
         scheduler = MipLRDecay(optimizer, lr_init=cfg.lr_init, lr_final=cfg.lr_final, max_steps=cfg.max_steps,
                                lr_delay_steps=cfg.lr_delay_steps, lr_delay_mult=cfg.lr_delay_mult)
         return {'optimizer': optimizer, 'lr_scheduler': scheduler}
@@ -81,6 +86,11 @@ class _RenderModule(nn.Module):
         train_loss = self.train_val_get(batch, batch_idx)
         opt.zero_grad()
         self.manual_backward(train_loss)
+        max_norm = getattr(self.config, 'max_grad_norm', None)
+        if max_norm is not None:
+            from .optim import clip_grad_norm_, own_max_norm
+            if own_max_norm(opt) is None:
+                clip_grad_norm_(self.parameters(), max_norm)
         opt.step()
         self.lr_schedulers().step()
         self._weights_changed()

@@ -27,6 +27,11 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     return ops.clip_grad_norm_(grads, max_norm, norm_type)
 
 
+def own_max_norm(optimizer):
+    """The norm that an optimizer clips at by itself (`AdamW` below with a max_norm), or None."""
+    return optimizer.max_norm if isinstance(optimizer, AdamW) else None
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay; arguments as torch.optim.AdamW's, and
 
@@ -156,13 +161,14 @@ class AdamW(torch.optim.Optimizer):
         if grad_ptrs is None:
             grads = self._as_params(grads, params)
             grad_ptrs = match(grads, params, False)
-        states = self._states(params, dtypes.strip(b'\0'))
+        half = bool(dtypes.strip(b'\0'))
+        states = self._states(params, half)
         state_ptrs = []
-        for k in ('exp_avg', 'exp_avg_sq', 'master'):
-            found = match([s.get(k) for s in states], params, True)
+        for k, of in (('exp_avg', states), ('exp_avg_sq', states), ('master', states if half else ())):
+            found = match([s.get(k) for s in of], params if of else [], True)
             if found is None:
                 raise RuntimeError(f'AdamW: state {k!r} has another order of dimensions than its parameter')
-            state_ptrs.append(found)
+            state_ptrs.append(found or None)
         step_device, step_ptrs, _, step_types, _ = lists().describe([s['step'] for s in states])
         if step_device != device or step_types.strip(b'\0'):
             raise RuntimeError('AdamW: state \'step\' must be fp32 on the parameters\' device')

@@ -118,9 +118,24 @@ def shard_range(n, rank, world_size):
     return lo, lo + base + (1 if rank < rem else 0)
 
 
+def _apply_gradients(model, bucket, optimizer, max_grad_norm):
+    """Clip the bucket (all-reduced: every rank holds the same sums and takes the same norm) and step the optimizer.
+    `nerf_amd.optim.AdamW` built with a max_norm clips as it reads the gradients, and the bucket is left as it is."""
+    from .optim import own_max_norm
+    own = own_max_norm(optimizer)
+    if own is None:
+        most = max_grad_norm if max_grad_norm is not None else getattr(model.config, 'max_grad_norm', None)
+        if most is not None:
+            from . import ops
+            ops.clip_grad_norm_(bucket.flat, most)
+    elif max_grad_norm is not None and float(max_grad_norm) != own:
+        raise ValueError(f'max_grad_norm={max_grad_norm}, but the optimizer clips at {own} by itself')
+    optimizer.step()
+
+
 def nerf_train_step(model, rays, pixels, optimizer, chunk=8192, world_size=1, global_mask_sum=None, scheduler=None,
-                    fused=True):
-    """fwd + bwd (+ all-reduce) + optimizer step on this rank's rays.
+                    fused=True, max_grad_norm=None):
+    """fwd + bwd (+ all-reduce) (+ clipping) + optimizer step on this rank's rays.
 
     The loss is sum(mask * err^2) / sum(mask) over the GLOBAL batch (util_modules.py:65), so each
     chunk contributes its masked squared-error sum divided by the global mask sum; gradients then
@@ -129,7 +144,10 @@ def nerf_train_step(model, rays, pixels, optimizer, chunk=8192, world_size=1, gl
     When the batch is one chunk and the model runs the bf16 chain, the step is the fixed launch sequence of
     `nerf_amd.stepper` (no autograd, persistent buffers, one backward chain and one weight-gradient pass for all
     levels); otherwise (`fused=False`, several chunks, the fp32 path, density noise) it goes through autograd
-    chunk by chunk.  Both accumulate into the same gradient bucket."""
+    chunk by chunk.  Both accumulate into the same gradient bucket.
+
+    `max_grad_norm` (default: the model's `config.max_grad_norm`, if it has one) clips the gradients of the whole batch by
+    their norm ahead of the optimizer; nothing is read back to the host."""
     bucket = grad_bucket(model)
     n = rays.origins.shape[0]
     if global_mask_sum is None:             # the denominator of the reference loss is the mask sum of the WHOLE batch
@@ -152,7 +170,7 @@ def nerf_train_step(model, rays, pixels, optimizer, chunk=8192, world_size=1, gl
                 early['hi'], early['work'] = hi, bucket.all_reduce(world_size, async_op=True, lo=0, hi=hi)
         total, _ = stepper.stepper_for(model, n).step(rays, pixels, global_mask_sum,
                                                       after_trunk=reduce_trunk if world_size > 1 else None)
-        return _finish_step(model, bucket, optimizer, scheduler, world_size, total, early)
+        return _finish_step(model, bucket, optimizer, scheduler, world_size, total, early, max_grad_norm)
     total = torch.zeros((), device=rays.origins.device)
     cwd = model.loss_function.coarse_weight_decay
     import contextlib
@@ -168,17 +186,17 @@ def nerf_train_step(model, rays, pixels, optimizer, chunk=8192, world_size=1, gl
             loss = cwd * sq[:-1].sum() + sq[-1]
             loss.backward()
             total += loss.detach()
-    return _finish_step(model, bucket, optimizer, scheduler, world_size, total)
+    return _finish_step(model, bucket, optimizer, scheduler, world_size, total, max_grad_norm=max_grad_norm)
 
 
-def _finish_step(model, bucket, optimizer, scheduler, world_size, total, early=None):
+def _finish_step(model, bucket, optimizer, scheduler, world_size, total, early=None, max_grad_norm=None):
     bucket.attach()
     lo = early.get('hi', 0) if early else 0           # floats 0 .. lo are already being reduced (nerf_train_step)
     work = bucket.all_reduce(world_size, async_op=True, lo=lo, hi=None if lo == 0 else bucket.flat.numel())
     for w in ((early or {}).get('work'), work):
         if w is not None:
             w.wait()            # orders the collective ahead of the optimizer kernels on the current stream
-    optimizer.step()
+    _apply_gradients(model, bucket, optimizer, max_grad_norm)
     if scheduler is not None:
         scheduler.step()
     model._weights_changed()
@@ -205,14 +223,14 @@ def allreduce_sum_shared_loss(x, world_size):
     return x if world_size <= 1 else _AllReduceSumSharedLoss.apply(x)
 
 
-def sar_train_step(model, batch, optimizer, rank=0, world_size=1, scheduler=None, fused=True, **draws):
+def sar_train_step(model, batch, optimizer, rank=0, world_size=1, scheduler=None, fused=True, max_grad_norm=None, **draws):
     """One SAR pulse, ray chunks dealt round-robin to the ranks (model.py:326-375 loops over them on one device).
 
     The reference ADDS the chunks' range profiles before the matched filter (model.py:371), and within a chunk
     the last ray written to a range bin wins; dealing whole chunks keeps both rules intact.  Each rank renders
     its chunks, the per-level profiles are SUM-all-reduced (nsam x 2 floats per level) ahead of the FFT and the
     per-pulse std, every rank evaluates the same loss, and the weight gradients -- partial sums over each
-    rank's chunks -- are SUM-all-reduced in one flat bucket."""
+    rank's chunks -- are SUM-all-reduced in one flat bucket.  `max_grad_norm` as in `nerf_train_step`."""
     ray_o, pan, tilt, mfilt, radii, near, far, mpp, pulse_data = batch
     bucket = grad_bucket(model)
     bucket.zero()
@@ -224,7 +242,7 @@ def sar_train_step(model, batch, optimizer, rank=0, world_size=1, scheduler=None
                                                                      mpp, pulse_data, **draws)
         bucket.attach()
         bucket.all_reduce(world_size)
-        optimizer.step()
+        _apply_gradients(model, bucket, optimizer, max_grad_norm)
         if scheduler is not None:
             scheduler.step()
         model._weights_changed()
@@ -236,7 +254,7 @@ def sar_train_step(model, batch, optimizer, rank=0, world_size=1, scheduler=None
         loss.backward()
     bucket.attach()
     bucket.all_reduce(world_size)
-    optimizer.step()
+    _apply_gradients(model, bucket, optimizer, max_grad_norm)
     if scheduler is not None:
         scheduler.step()
     model._weights_changed()
@@ -250,21 +268,21 @@ class GraphedSarStep:
     about a hundred short launches -- samplers, encoders, chain kernels, scatter, FFTs, loss, the backward of all of
     them, AdamW, weight repack -- and a step issued launch by launch is bound by the host; replaying the captured
     graph leaves only the kernels.  Needs one rank, `config.check_range = False` (the range check reads a status
-    word back, which a capture cannot do) and an optimizer built with `capturable=True`.  The learning rate must be
-    a device tensor for a replay to see a new value (a Python number is baked into the captured kernels' arguments):
-    a float `lr` of a parameter group is replaced by a one-element device tensor here, before the warm-up steps, and
+    word back, which a capture cannot do) and an optimizer built with `capturable=True` (`nerf_amd.optim.AdamW` always
+    is).  The learning rate must be a device tensor for a replay to see a new value (a Python number is baked into the
+    captured kernels' arguments): a float `lr` of a parameter group is replaced by a one-element device tensor here, before the warm-up steps, and
     `step(lr=...)` / `set_lr` write into it (the reference steps MipLRDecay after every optimizer step,
     model.py:389-393).  The beam offsets are
     drawn on the device (the reference draws them on the host, model.py:319-320: same distribution, another
     stream of numbers); every replay draws afresh.  The `warmup` eager runs that precede the capture are real
     optimizer steps."""
 
-    def __init__(self, model, batch, optimizer, warmup=3):
+    def __init__(self, model, batch, optimizer, warmup=3, max_grad_norm=None):
         if getattr(model.config, 'check_range', True):
             raise ValueError('GraphedSarStep: set config.check_range = False (the check synchronises the stream)')
         if not all(g.get('capturable', False) for g in optimizer.param_groups):
             raise ValueError('GraphedSarStep: build the optimizer with capturable=True')
-        self.model, self.optimizer = model, optimizer
+        self.model, self.optimizer, self.max_grad_norm = model, optimizer, max_grad_norm
         dev = model.device
         for g in optimizer.param_groups:        # see the class comment: only a tensor lr reaches a replay
             if not torch.is_tensor(g['lr']):
@@ -287,7 +305,7 @@ class GraphedSarStep:
         m = self.model
         az_el = [(torch.randn(m.rays_per_chunk, device=m.device) * SAR_AZ_SIGMA,
                   torch.randn(m.rays_per_chunk, device=m.device) * SAR_EL_SIGMA) for _ in range(m.num_ray_iters)]
-        return sar_train_step(m, self.batch, self.optimizer, az_el=az_el)
+        return sar_train_step(m, self.batch, self.optimizer, max_grad_norm=self.max_grad_norm, az_el=az_el)
 
     def set_lr(self, lr):
         """Write `lr` (a number, or one per parameter group) into the optimizer's tensor learning rates."""
