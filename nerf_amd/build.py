@@ -16,7 +16,10 @@ LIBDIR = os.path.join(HERE, 'lib')
 OBJDIR = os.path.join(LIBDIR, 'obj')
 LIB = os.path.join(LIBDIR, 'libnerf_amd.so')
 
-COMMON = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall', '-Wno-unused-function']
+# (no packed fp32 instructions: the compiler forms them from ordinary float code, and some of their forms have given wrong
+# results on this hardware)
+COMMON = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall', '-Wno-unused-function',
+          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # translation unit -> extra flags.  The sampling / compositing kernels must round every fp32
 # operation separately (parity with the reference's op-by-op torch arithmetic).
 # mlp_bf16.hip is compiled in parts (-DNERF_NET_PART=p): the chain kernels of each large network geometry take
@@ -27,7 +30,7 @@ UNITS = {
     'composite.o': ('composite.hip', ['-ffp-contract=off']),
     'sar_pulse.o': ('sar_pulse.hip', []),
     'gemm_f32.o': ('gemm_f32.hip', []),
-    'optimizer.o': ('optimizer.hip', ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']),
+    'optimizer.o': ('optimizer.hip', []),
     # VGPR-form matrix-core instructions where an accumulator tile lives in the vector registers: the outputs of the
     # larger launches exceed the 256 accumulation registers, and the default form copies such tiles in and out
     # of them around every product (layer 4's launch: 1.10 -> 0.86 ms)
