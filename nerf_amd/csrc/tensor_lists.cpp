@@ -28,6 +28,13 @@ int type_code(const at::Tensor& t) {
 
 bool dense(const at::Tensor& t) { return t.unsafeGetTensorImpl()->is_non_overlapping_and_dense_or_false(); }
 
+// Whether the entries of two tensors of one shape lie in the same order (dimensions of one entry have no say in it).
+bool same_order(const at::Tensor& a, const at::Tensor& b) {
+    for (int64_t d = 0; d < a.dim(); ++d)
+        if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return a.numel() == 0;
+    return true;
+}
+
 const at::Tensor* tensor_at(PyObject* list, Py_ssize_t i) {
     PyObject* o = PyList_GET_ITEM(list, i);
     if (!THPVariable_Check(o)) {
@@ -72,7 +79,7 @@ PyObject* describe(PyObject*, PyObject* list) {
         } else {
             device = t->get_device();
             all_dense = all_dense && dense(*t);
-            ((uint64_t*)PyBytes_AS_STRING(ptrs))[i] = (uint64_t)t->const_data_ptr();
+            ((uint64_t*)PyBytes_AS_STRING(ptrs))[i] = (uint64_t)t->mutable_data_ptr();
             ((int64_t*)PyBytes_AS_STRING(numels))[i] = t->numel();
             ((int32_t*)PyBytes_AS_STRING(types))[i] = type_code(*t);
         }
@@ -95,7 +102,7 @@ PyObject* match(PyObject*, PyObject* args) {
     }
     PyObject* ptrs = PyBytes_FromStringAndSize(nullptr, n * 8);
     if (!ptrs) return nullptr;
-    bool same_order = true;
+    bool ordered = true;
     for (Py_ssize_t i = 0; i < n; ++i) {
         uint64_t* at = (uint64_t*)PyBytes_AS_STRING(ptrs) + i;
         if (PyList_GET_ITEM(list, i) == Py_None) {
@@ -112,10 +119,10 @@ PyObject* match(PyObject*, PyObject* args) {
             return PyErr_Format(PyExc_RuntimeError, "expected %s tensors of their parameters' shape and device",
                                 fp32 ? "fp32" : "same-type");
         }
-        same_order = same_order && (t->strides() == l->strides() || (t->is_contiguous() && l->is_contiguous()));
-        *at = (uint64_t)t->const_data_ptr();
+        ordered = ordered && same_order(*t, *l);
+        *at = (uint64_t)t->mutable_data_ptr();
     }
-    if (!same_order) {
+    if (!ordered) {
         Py_DECREF(ptrs);
         Py_RETURN_NONE;
     }

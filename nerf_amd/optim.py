@@ -40,8 +40,8 @@ class AdamW(torch.optim.Optimizer):
     norm_type        2, 1 or inf.
     skip_nonfinite   a step whose gradient norm is infinite or NaN leaves parameters, moments and step counters as they are.
 
-    `grad_norm` holds the norm of the last step (a 0-d fp32 tensor on the device; None before the first, and without
-    max_norm or skip_nonfinite).  Parameters are fp32, bf16 or fp16, on one HIP device, their gradients of the same type.
+    `grad_norm` holds the norm of the last step (a 0-d fp32 tensor on the device, which the replays of a captured step
+    write again; None before the first, and without max_norm or skip_nonfinite).  Parameters are fp32, bf16 or fp16, on one HIP device, their gradients of the same type.
     The moments are fp32 whatever the parameters are, and a 16-bit parameter has an fp32 master weight in the state
     ('master'), of which it is the rounding.  The step counters live on the device, so a captured step counts on with
     every replay; the learning rate of a group may be an fp32 device tensor, which a replay reads afresh.  The state is
@@ -62,6 +62,10 @@ class AdamW(torch.optim.Optimizer):
         self.norm_type, self.skip_nonfinite = float(norm_type), bool(skip_nonfinite)
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, capturable=True))
+
+    def __getstate__(self):         # (copies and pickles: the base class names what it keeps)
+        return dict(super().__getstate__(), max_norm=self.max_norm, norm_type=self.norm_type,
+                    skip_nonfinite=self.skip_nonfinite, _kind=self._kind, grad_norm=None)
 
     def __setstate__(self, state):
         super().__setstate__(state)

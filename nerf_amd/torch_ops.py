@@ -18,6 +18,9 @@ capture works unchanged.  All take contiguous fp32 tensors on one HIP device, fl
                                                                                           w.r.t. the weights)
     torch.ops.nerf_amd.mlp_bwd(weights, geom, M, g_density, g_rgb, g_angle, outs, acts)   the input-gradient chain
     torch.ops.nerf_amd.mlp_wgrad(weights, geom, M, acts, dys)                             the weight gradients
+    torch.ops.nerf_amd.grad_norm(tensors, norm_type)                                      the norm of a list of gradients
+    torch.ops.nerf_amd.clip_grad_norm_(tensors, max_norm, norm_type)                      scales them in place -> the norm
+                                                                                          (lists of fp32 / bf16 / fp16)
 """
 from typing import List, Optional, Sequence, Tuple
 
@@ -344,3 +347,25 @@ def _mlp_backward(ctx, g_density, g_rgb, g_angle, _g_ln, _g_acts):
 
 
 mlp_fwd.register_autograd(_mlp_backward, setup_context=_mlp_setup)
+
+
+# ---- gradient norm and clipping (csrc/optimizer.hip) ----------------------------------------------------------------
+
+@torch.library.custom_op('nerf_amd::grad_norm', mutates_args=())
+def grad_norm(tensors: Sequence[Tensor], norm_type: float) -> Tensor:
+    return ops.grad_norm(tensors, norm_type)
+
+
+@grad_norm.register_fake
+def _(tensors, norm_type):
+    return tensors[0].new_empty((), dtype=torch.float32) if len(tensors) else torch.empty((), device='cuda')
+
+
+@torch.library.custom_op('nerf_amd::clip_grad_norm_', mutates_args=('tensors',))
+def clip_grad_norm_(tensors: Sequence[Tensor], max_norm: float, norm_type: float) -> Tensor:
+    return ops.clip_grad_norm_(tensors, max_norm, norm_type)
+
+
+@clip_grad_norm_.register_fake
+def _(tensors, max_norm, norm_type):
+    return tensors[0].new_empty((), dtype=torch.float32) if len(tensors) else torch.empty((), device='cuda')

@@ -438,7 +438,9 @@ def test_orders_of_parameters_and_gradients():
     b.grad = torch.randn(30, 50, device='cuda', generator=g).t()
     c = torch.nn.Parameter(torch.randn(1, 64, device='cuda', generator=g))
     c.grad = torch.randn(64, 1, device='cuda', generator=g).t()
-    ps = [a, b, c]
+    d = torch.nn.Parameter(torch.randn(40, device='cuda', generator=g).as_strided((3, 1, 4), (1, 7, 3)))
+    d.grad = torch.randn(3, 1, 4, device='cuda', generator=g)
+    ps = [a, b, c, d]
     from nerf_amd import optim
     opt = optim.AdamW(ps, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD)
     was = [(p.detach().clone(), p.grad.clone(), torch.zeros_like(p), torch.zeros_like(p)) for p in ps]
@@ -580,3 +582,26 @@ def test_more_than_2_to_the_31_elements():
     del g
     gc.collect()
     torch.cuda.empty_cache()
+
+
+def test_custom_ops():
+    import nerf_amd.torch_ops  # noqa: F401
+    K = torch.ops.nerf_amd
+    for sizes in ('network', 'short'):
+        ts = make(SIZES[sizes], torch.float32)
+        near_norm(K.grad_norm(ts, 1.0), norm64(ts, 1.0))
+        was = [t.double() for t in ts]
+        check_clipped(ts, was, 0.1, 2.0, K.clip_grad_norm_(ts, 0.1, 2.0))
+    ts = make([33, 1000], torch.bfloat16)
+    torch.library.opcheck(K.grad_norm.default, (ts, 2.0), test_utils=('test_schema', 'test_faketensor'))
+    torch.library.opcheck(K.clip_grad_norm_.default, (ts, 1.0, 2.0), test_utils=('test_schema', 'test_faketensor'))
+
+    def scaled(ts):
+        n = K.clip_grad_norm_(ts, 0.5, 2.0)
+        return [t * 2 for t in ts], n + K.grad_norm(ts, math.inf)
+    a = make(SIZES['network'], torch.float32)
+    b = [t.clone() for t in a]
+    ys, n = torch.compile(scaled, fullgraph=True, backend='aot_eager')(a)
+    zs, m = scaled(b)
+    assert torch.equal(n, m) and all(torch.equal(y, z) for y, z in zip(ys, zs))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -145,6 +145,8 @@ def test_list_reader():
     assert read(L.match([torch.zeros(1, 5).t().contiguous().t()], [torch.zeros(1, 5)], False)) != [0]
     assert L.match([a], [b], False) is None
     assert L.match([b], [b], True) is not None
+    odd = torch.zeros(40).as_strided((3, 1, 4), (1, 7, 3))
+    assert L.match([torch.zeros_like(odd)], [odd], False) is not None
     for x, y, fp32 in ((a, torch.zeros(4, 3), False), (a.half(), a, False), (a.half(), a.half(), True)):
         with pytest.raises(RuntimeError, match='shape'):
             L.match([x], [y], fp32)
@@ -179,3 +181,15 @@ def test_state_dict_of_the_other_optimizer():
     moments['state'][1]['exp_avg'] = torch.full((5,), 1.0 + 2.0 ** -20)
     mine.load_state_dict(moments)
     assert torch.equal(mine.state[b]['exp_avg'], torch.full((5,), 1.0 + 2.0 ** -20))
+
+
+def test_copies_of_an_optimizer():
+    import copy
+    import pickle
+    p = torch.nn.Parameter(CPU.clone())
+    opt = optim.AdamW([p], lr=0.25, max_norm=2.0, norm_type=1, skip_nonfinite=True)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert (other.max_norm, other.norm_type, other.skip_nonfinite, other.grad_norm) == (2.0, 1.0, True, None)
+        assert other._kind == opt._kind and other.param_groups[0]['lr'] == 0.25
+        assert optim.own_max_norm(other) == 2.0
+    assert optim.own_max_norm(torch.optim.AdamW([p])) is None
