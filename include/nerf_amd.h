@@ -414,7 +414,8 @@ int nerf_grad_norm(const void* const* grads, const int64_t* numel, const int32_t
 
 /* g *= min(1, max_norm / (norm + 1e-6)), in place, for every entry of every tensor; norm[1] receives the norm before.
  * Products are taken in fp32 and rounded once to the tensor's type.  A NaN norm makes every entry NaN; with an infinite
- * one finite entries become 0 and infinite ones NaN.  The tensors must not share memory (NERF_ERR_ARG). */
+ * one finite entries become 0 and infinite ones NaN.  The tensors must not share memory (NERF_ERR_ARG; a list that does
+ * not ascend in memory is sorted in temporary host memory to see). */
 int nerf_clip_grad_norm(void* const* grads, const int64_t* numel, const int32_t* dtype, int n_tensors, int norm_kind,
                         double max_norm, void* workspace, int64_t workspace_bytes, float* norm, void* stream);
 
