@@ -95,89 +95,42 @@ class AdamW(torch.optim.Optimizer):
                     del g[k]
             g['capturable'] = True
 
-    @staticmethod
-    def _not_captured():
+    def _init_state(self, params):
+        """Lay out the state of parameters that have none, or no master (the state of an optimizer that keeps none)."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('AdamW: run one step ahead of a graph capture (it lays out the optimizer state; captured, '
                                'every replay would clear it)')
-
-    def _master_of(self, p):
-        self._not_captured()
-        return p.detach().to(torch.float32, memory_format=torch.preserve_format)
-
-    def _init_state(self, params):
-        self._not_captured()
         steps = torch.zeros(len(params), dtype=torch.float32, device=params[0].device)
         for i, p in enumerate(params):
             st = self.state[p]
-            st['step'] = steps[i]
-            st['exp_avg'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
-            st['exp_avg_sq'] = torch.zeros_like(st['exp_avg'])
+            like = dict(dtype=torch.float32, memory_format=torch.preserve_format)
+            if not st:
+                st['step'] = steps[i]
+                st['exp_avg'] = torch.zeros_like(p, **like)
+                st['exp_avg_sq'] = torch.zeros_like(p, **like)
             if p.dtype != torch.float32:
-                st['master'] = self._master_of(p)
+                st['master'] = p.detach().to(**like)
 
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        params, grads, counts = [], [], []
-        for group in self.param_groups:
-            before = len(params)
-            for p in group['params']:
-                g = p.grad
-                if g is not None:
-                    params.append(p)
-                    grads.append(g)
-            counts.append(len(params) - before)
-        clips = self.max_norm is not None or self.skip_nonfinite
+        lists_of = [g['params'] for g in self.param_groups]
+        found = lists().optimizer(lists_of, self.state)
+        if type(found) is list:
+            ops.list_call(found[0].get_device(), lambda _: self._init_state(found))
+            found = lists().optimizer(lists_of, self.state)
+        device, params, _, counts, *arrays = found
         if params:
-            table = lists().describe(params)
-            if not table[-1]:
-                raise RuntimeError('AdamW: expected dense parameters (no gaps, no broadcast dimensions)')
-            ops.list_call(table[0], lambda st: self._launch(params, grads, counts, clips, table, st))
+            ops.list_call(device, lambda st: self._launch(device, len(params), memoryview(counts).cast('i'), arrays, st))
             torch.autograd.graph.increment_version(params)      # (the kernels write behind autograd's back)
-        elif clips:
-            p = next((p for g in self.param_groups for p in g['params']), None)
-            self.grad_norm = torch.zeros((), device=p.device if p is not None else None)
+        elif self.max_norm is not None or self.skip_nonfinite:
+            self.grad_norm = torch.zeros((), device=next((p.device for ps in lists_of for p in ps), None))
         return loss
 
-    def _states(self, params, half):
-        states = [self.state[p] for p in params]
-        if {} in states:
-            self._init_state([p for p, st in zip(params, states) if not st])
-        if half:
-            for p, st in zip(params, states):
-                if 'master' not in st and p.dtype != torch.float32:     # (the state of an optimizer that keeps none)
-                    st['master'] = self._master_of(p)
-        return states
-
-    @torch.no_grad()
-    def _as_params(self, tensors, params):
-        """The tensors laid out as their parameters are (another order of the same entries)."""
-        return [torch.empty_like(p, memory_format=torch.preserve_format).copy_(t) for t, p in zip(tensors, params)]
-
-    def _launch(self, params, grads, counts, clips, table, st):
-        L, match = lib(), lists().match
-        n = len(params)
-        device, ptrs, numels, dtypes, _ = table
-        grad_ptrs = match(grads, params, False)
-        if grad_ptrs is None:
-            grads = self._as_params(grads, params)
-            grad_ptrs = match(grads, params, False)
-        half = bool(dtypes.strip(b'\0'))
-        states = self._states(params, half)
-        state_ptrs = []
-        for k, of in (('exp_avg', states), ('exp_avg_sq', states), ('master', states if half else ())):
-            found = match([s.get(k) for s in of], params if of else [], True)
-            if found is None:
-                raise RuntimeError(f'AdamW: state {k!r} has another order of dimensions than its parameter')
-            state_ptrs.append(found or None)
-        step_device, step_ptrs, _, step_types, _ = lists().describe([s['step'] for s in states])
-        if step_device != device or step_types.strip(b'\0'):
-            raise RuntimeError('AdamW: state \'step\' must be fp32 on the parameters\' device')
-        arrays = (ptrs, grad_ptrs, *state_ptrs, step_ptrs, numels, dtypes)
-        t = AdamwTensors(n, *arrays)
+    def _launch(self, device, n, counts, arrays, st):
+        L = lib()
         groups = (AdamwGroup * len(counts))()
         for c, count, g in zip(groups, counts, self.param_groups):
             lr = g['lr']
@@ -195,10 +148,11 @@ class AdamW(torch.optim.Optimizer):
                 c.lr = float(lr)
             c.beta1, c.beta2 = g['betas']
             c.eps, c.weight_decay = g['eps'], g['weight_decay']
+        clips = self.max_norm is not None or self.skip_nonfinite
         nbytes = L.nerf_grad_workspace_bytes(n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device='cuda')
         norm = torch.empty((), dtype=torch.float32, device='cuda') if clips else None
-        check(L.nerf_adamw_step(ctypes.byref(t), groups, len(counts), self._kind if clips else 0,
+        check(L.nerf_adamw_step(ctypes.byref(AdamwTensors(n, *arrays)), groups, len(counts), self._kind if clips else 0,
                                 float('inf') if self.max_norm is None else self.max_norm, int(self.skip_nonfinite),
                                 ws.data_ptr(), nbytes, norm.data_ptr() if clips else None, st))
         if clips:

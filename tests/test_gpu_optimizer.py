@@ -207,10 +207,13 @@ def test_refusals_on_the_device():
         opt.step()
     opt = optim.AdamW([p])
     opt.state[p] = dict(step=torch.zeros(()), exp_avg=torch.zeros_like(p), exp_avg_sq=torch.zeros_like(p))
-    with pytest.raises(RuntimeError, match='HIP device'):
+    with pytest.raises(RuntimeError, match='step'):
         opt.step()
     opt.state[p] = dict(step=torch.zeros((), device='cuda'), exp_avg=torch.zeros(4), exp_avg_sq=torch.zeros_like(p))
-    with pytest.raises(RuntimeError, match='shape and device'):
+    with pytest.raises(RuntimeError, match='shape, order and device'):
+        opt.step()
+    opt.state[p] = dict(step=torch.zeros((), device='cuda'), exp_avg=torch.zeros_like(p))
+    with pytest.raises(RuntimeError, match='exp_avg_sq'):
         opt.step()
     opt.state[p] = dict(step=torch.zeros((), device='cuda', dtype=torch.bfloat16), exp_avg=torch.zeros_like(p),
                         exp_avg_sq=torch.zeros_like(p))

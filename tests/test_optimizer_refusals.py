@@ -139,19 +139,14 @@ def test_list_reader():
         L.describe([torch.zeros(3, 3).to_sparse()])
     with pytest.raises(RuntimeError, match='strided'):
         L.describe([torch.zeros(3, dtype=torch.complex64).conj().imag])
-    a, b = torch.zeros(3, 4), torch.zeros(4, 3).t()
-    read = lambda x: array('Q', x).tolist()         # noqa: E731
-    assert read(L.match([a, None], [a, b], False)) == [a.data_ptr(), 0]
-    assert read(L.match([torch.zeros(1, 5).t().contiguous().t()], [torch.zeros(1, 5)], False)) != [0]
-    assert L.match([a], [b], False) is None
-    assert L.match([b], [b], True) is not None
-    odd = torch.zeros(40).as_strided((3, 1, 4), (1, 7, 3))
-    assert L.match([torch.zeros_like(odd)], [odd], False) is not None
-    for x, y, fp32 in ((a, torch.zeros(4, 3), False), (a.half(), a, False), (a.half(), a.half(), True)):
-        with pytest.raises(RuntimeError, match='shape'):
-            L.match([x], [y], fp32)
-    with pytest.raises(ValueError):
-        L.match([a], [], False)
+    for bad in ((), ([], {}, 1), ((), {}), ([()], {}), ([3], {})):
+        with pytest.raises(TypeError):
+            L.optimizer(*bad)
+    p = torch.nn.Parameter(CPU.clone())
+    assert L.optimizer([[p], []], {}) == (-1, [], [], b'\0' * 8, b'', b'', b'', b'', None, b'', b'', b'')
+    p.grad = torch.ones(8)
+    with pytest.raises(RuntimeError, match='HIP device'):
+        L.optimizer([[p]], {})
 
 
 def test_unsupported_optimizer_states():
