@@ -41,11 +41,13 @@ class AdamW(torch.optim.Optimizer):
     skip_nonfinite   a step whose gradient norm is infinite or NaN leaves parameters, moments and step counters as they are.
 
     `grad_norm` holds the norm of the last step (a 0-d fp32 tensor on the device, which the replays of a captured step
-    write again; None before the first, and without max_norm or skip_nonfinite).  Parameters are fp32, bf16 or fp16, on one HIP device, their gradients of the same type.
-    The moments are fp32 whatever the parameters are, and a 16-bit parameter has an fp32 master weight in the state
-    ('master'), of which it is the rounding.  The step counters live on the device, so a captured step counts on with
-    every replay; the learning rate of a group may be an fp32 device tensor, which a replay reads afresh.  The state is
-    laid out by the first step, which therefore cannot be a captured one."""
+    write again; None before the first, and without max_norm or skip_nonfinite).
+
+    Parameters are fp32, bf16 or fp16, on one HIP device, their gradients of the same type.  The moments are fp32 whatever
+    the parameters are, and a 16-bit parameter has an fp32 master weight in the state ('master'), of which it is the
+    rounding; a parameter that something else writes is taken as it is, and its master follows.  The step counters live on
+    the device, so a captured step counts on with every replay; the learning rate of a group may be an fp32 device tensor,
+    which a replay reads afresh.  The state is laid out by the first step, which therefore cannot be a captured one."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, norm_type=2.0,
                  skip_nonfinite=False):
@@ -117,7 +119,7 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         lists_of = [g['params'] for g in self.param_groups]
-        found = lists().optimizer(lists_of, self.state)
+        found = lists().optimizer(lists_of, self.state)     # (holds copies of reordered gradients: kept to the end)
         if type(found) is list:
             ops.list_call(found[0].get_device(), lambda _: self._init_state(found))
             found = lists().optimizer(lists_of, self.state)

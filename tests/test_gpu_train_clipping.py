@@ -168,3 +168,59 @@ def test_captured_sar_pulse_step(own):
         assert float(opt.state[first]['step']) == 3 + k
         same = all(torch.equal(a, b) for a, b in zip(was, weights(m)))
         assert same is (k == 2) and all(torch.isfinite(w).all() for w in weights(m))
+
+
+def _rank(rank, port, own, q):
+    import os
+
+    import torch.distributed as dist
+
+    from nerf_amd import optim
+    from nerf_amd.train import grad_bucket, nerf_train_step, shard_range
+    from nerf_amd.utils import namedtuple_map
+    os.environ.update(MASTER_ADDR='127.0.0.1', MASTER_PORT=str(port))
+    dist.init_process_group('gloo', rank=rank, world_size=2)
+    m, (rays, pixels) = model_and_batch(n=97)
+    lo, hi = shard_range(97, rank, 2)
+    shard = namedtuple_map(lambda t: t[lo:hi], rays)
+    opt = (optim.AdamW(m.parameters(), lr=1e-3, max_norm=0.01) if own else
+           torch.optim.SGD([p for p in m.parameters() if p.requires_grad], lr=0.1))
+    for _ in range(3):
+        nerf_train_step(m, shard, pixels[lo:hi], opt, chunk=97, world_size=2, max_grad_norm=0.01)
+    torch.cuda.synchronize()
+    norm = float(opt.grad_norm) if own else 0.0
+    q.put((rank, norm, norm64([grad_bucket(m).flat]), torch.cat([w.reshape(-1) for w in weights(m)]).cpu().numpy()))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize('own', [True, False])
+def test_two_ranks_clip_alike(own):
+    """Two ranks (sharing the GPU, gloo between them) clip the all-reduced gradients by the same norm bit for bit: after
+    three steps on shards of different sizes their weights are still the same."""
+    import socket
+
+    import numpy as np
+    import torch.multiprocessing as mp
+    s = socket.socket()
+    s.bind(('127.0.0.1', 0))
+    port = s.getsockname()[1]
+    s.close()
+    ctx = mp.get_context('spawn')
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_rank, args=(r, port, own, q)) for r in range(2)]
+    for pr in procs:
+        pr.start()
+    try:
+        got = [q.get(timeout=100) for _ in range(2)]
+    finally:
+        for pr in procs:
+            pr.join(20)
+            if pr.is_alive():
+                pr.kill()
+    assert all(pr.exitcode == 0 for pr in procs)
+    assert got[0][1:3] == got[1][1:3] and np.array_equal(got[0][3], got[1][3]) and np.isfinite(got[0][3]).all()
+    if own:
+        assert abs(got[0][1] - got[0][2]) <= got[0][2] * 2 * U
+    else:
+        assert got[0][2] <= 0.01 * (1 + 4 * U)
