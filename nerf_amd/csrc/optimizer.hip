@@ -27,8 +27,8 @@ constexpr int kThreads = 256;
 // How a kernel's launches are cut: at most `groups` workgroups, and chunks of `least` elements (one access per lane) while
 // the list is short, so that every compute unit gets some, up to `most` for a long one.  What the workgroups touch at one
 // time (groups x chunk, in each of the tensors' arrays) is kept to a few megabytes: AdamW over 1e8 fp32 parameters took
-// 702 us with 2048 workgroups and chunks of 16384, 604 with 1024 and 16384, 567 with 1024 and 4096, 548 with 768 and
-// 2048 (and 725 with 512 and 1024, where the chunks' ends cost more); the norm of 4.3 GB 770 us with 2048 and 16384, 736
+// 702 us with 2048 workgroups and chunks of 16384, 604 with 1024 and 16384, 567 with 1024 and 4096, 547 with 768 and
+// 2048, 531 with 512 and 2048 (582 with 640, 588 with 256 and twice the loads under way); the norm of 4.3 GB 770 us with 2048 and 16384, 736
 // with 1024, the same at 1024 for chunks of 8192 to 32768; its inner loop wants four accesses per lane and chunk (5e8
 // bf16 elements in chunks of 4096: 190 us, of 16384: 128).
 struct Cut {
@@ -37,7 +37,7 @@ struct Cut {
 constexpr int kNormGroups = 1024;
 constexpr Cut norm_cut(int size) { return {kNormGroups, 4096 / size, 32768 / size}; }
 constexpr Cut scale_cut(int size) { return {1024, 4096 / size, 16384 / size}; }
-constexpr Cut adam_cut(int) { return {768, 1024, 2048}; }
+constexpr Cut adam_cut(int) { return {512, 1024, 2048}; }
 
 // Accesses past the caches (non-temporal ones), in bytes of what a call reads and writes.  A norm that nothing follows:
 // 4.3 GB 613 us against 735 through the caches, 120 MB 25.1 against 28.4 and 40 MB 11.8 either way; 120 MB that were
@@ -323,9 +323,9 @@ __device__ __forceinline__ float weight_of(T p, float master) {
 // than the rounding of the rounded sum: the value has to exist in 32 bits first.
 __device__ __forceinline__ void keep_rounded(float& x) { asm("" : "+v"(x)); }
 
-// Bound by memory: 28 bytes per fp32 parameter and 30 per 16-bit one; 1e8 fp32 parameters in 128 tensors 475 us of 546
-// with the norm, 5.9 TB/s; 2.5e8 bf16 ones in 300 tensors 1390 of 1470, 5.4 TB/s (six launches, about 8 us each to drain
-// and fill).  Division and square root are the correctly rounded ones; they hide behind the accesses.
+// Bound by memory: 28 bytes per fp32 parameter and 30 per 16-bit one; 1e8 fp32 parameters in 128 tensors 529 us with the
+// norm, 3.2 GB at 6.0 TB/s; 2.5e8 bf16 ones in 300 tensors 1400, 8.0 GB at 5.7 TB/s (three launches of the norm and six of
+// this, about 8 us each to drain and fill).  Division and square root are the correctly rounded ones; they hide behind the accesses.
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(kThreads) void adamw(AdamTable tab, Clip clip, AdamArgs a, const float* steps) {
     constexpr bool kMaster = sizeof(T) == 2;
