@@ -492,6 +492,41 @@ def test_another_stream_and_the_same_bits():
     assert all(torch.equal(x, want) for x in got)
 
 
+def test_two_threads_at_once():
+    """Two threads on streams of their own, each clipping its gradients and stepping its optimizer, against the same calls
+    one after another."""
+    import threading
+
+    from nerf_amd import ops, optim
+
+    def calls(seed, out):
+        ps = params_of(SIZES['network'], torch.float32, seed=seed)
+        opt = optim.AdamW(ps, lr=LR, max_norm=0.3)
+        norms = []
+        for _ in range(40):
+            norms.append(ops.clip_grad_norm_([p.grad for p in ps], 2.0 - 0.02 * len(norms)))
+            opt.step()
+            norms.append(opt.grad_norm)
+        out[seed] = ([float(n) for n in norms], [p.detach().clone() for p in ps])
+
+    def on_stream(seed, out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            calls(seed, out)
+            torch.cuda.current_stream().synchronize()
+    want, got = {}, {}
+    for seed in (20, 30):
+        calls(seed, want)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=on_stream, args=(seed, got)) for seed in (20, 30)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for seed in (20, 30):
+        assert got[seed][0] == want[seed][0]
+        assert all(torch.equal(a, b) for a, b in zip(got[seed][1], want[seed][1]))
+
+
 def test_captured_steps_count_on():
     """Two graphs of one optimizer, replayed in turn with eager work between, against the same steps taken eagerly."""
     from nerf_amd import optim
