@@ -75,13 +75,26 @@ class AdamW(torch.optim.Optimizer):
             g['capturable'] = True
 
     def load_state_dict(self, state_dict):
-        """A state dict of this class or of torch.optim.AdamW (without amsgrad / maximize)."""
-        for g in state_dict['param_groups']:
-            if g.get('amsgrad') or g.get('maximize'):
-                raise ValueError('AdamW: amsgrad and maximize are not supported')
-        super().load_state_dict(state_dict)
-        # The base class gives floating-point state the parameter's type and may leave step counters on the host: the
-        # moments and masters are fp32 here, and the counters live beside them.
+        """A state dict of this class or of torch.optim.AdamW (without amsgrad / maximize), with the registered hooks as they
+        are everywhere: the pre-hooks decide what is loaded, the post-hooks see it laid out."""
+        loaded = {}
+
+        def check_loaded(_, sd):                # behind the other pre-hooks, each of which may put another dict in its place
+            for g in sd['param_groups']:
+                if g.get('amsgrad') or g.get('maximize'):
+                    raise ValueError('AdamW: amsgrad and maximize are not supported')
+            loaded.update(sd)
+        hooks = (self.register_load_state_dict_pre_hook(check_loaded),
+                 self.register_load_state_dict_post_hook(lambda _: self._lay_out(loaded), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    def _lay_out(self, state_dict):
+        """What the base class has loaded, as the kernels take it.  It gives floating-point state the parameter's type and may
+        leave step counters on the host: the moments and masters are fp32 here, and the counters live beside them."""
         ids = [i for g in state_dict['param_groups'] for i in g['params']]
         for i, p in zip(ids, [p for g in self.param_groups for p in g['params']]):
             saved = state_dict['state'].get(i)

@@ -1,0 +1,70 @@
+"""Loading the AdamW step's state (no GPU needed)."""
+import pytest
+import torch
+
+from nerf_amd import optim
+
+
+def two():
+    return [torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4))]
+
+
+def saved(a, b):
+    """The state dict of an optimizer whose two parameters' moments are `a` and `b` throughout."""
+    ps = two()
+    opt = torch.optim.AdamW(ps)
+    for p, x in zip(ps, (a, b)):
+        opt.state[p] = dict(step=torch.tensor(3.0), exp_avg=torch.full((4,), x), exp_avg_sq=torch.full((4,), x * x))
+    return opt.state_dict()
+
+
+def swapped(state_dict):
+    """The same state dict for the parameters in the other order."""
+    state = state_dict['state']
+    return dict(state_dict, state={0: state[1], 1: state[0]})
+
+
+@pytest.mark.parametrize('cls', [optim.AdamW, torch.optim.AdamW])
+def test_a_pre_hook_decides_what_is_loaded(cls):
+    ps = two()
+    opt = cls(ps)
+    opt.register_load_state_dict_pre_hook(lambda _, sd: swapped(sd))
+    given = saved(0.2, 0.1)
+    opt.load_state_dict(given)
+    for p, x in zip(ps, (0.1, 0.2)):
+        assert torch.equal(opt.state[p]['exp_avg'], torch.full((4,), x))
+        assert torch.equal(opt.state[p]['exp_avg_sq'], torch.full((4,), x * x))
+        assert float(opt.state[p]['step']) == 3.0
+    opt.load_state_dict(given)              # (a second time: nothing of the first is left behind)
+    assert torch.equal(opt.state[ps[0]]['exp_avg'], torch.full((4,), 0.1))
+
+
+def test_a_pre_hook_on_16_bit_parameters_keeps_the_moments_in_32():
+    ps = [torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16)) for _ in range(2)]
+    opt = optim.AdamW(ps)
+    opt.register_load_state_dict_pre_hook(lambda _, sd: swapped(sd))
+    opt.load_state_dict(saved(1.0 + 2.0 ** -20, 3.0))
+    assert torch.equal(opt.state[ps[1]]['exp_avg'], torch.full((4,), 1.0 + 2.0 ** -20))
+
+
+def test_a_pre_hook_may_bring_what_is_refused():
+    opt = optim.AdamW(two())
+    other = torch.optim.AdamW(two(), amsgrad=True).state_dict()
+    opt.register_load_state_dict_pre_hook(lambda _, sd: other)
+    before = opt.state_dict()
+    with pytest.raises(ValueError, match='amsgrad'):
+        opt.load_state_dict(saved(0.1, 0.2))
+    assert opt.state_dict() == before
+
+
+@pytest.mark.parametrize('cls', [optim.AdamW, torch.optim.AdamW])
+def test_a_post_hook_has_the_last_word(cls):
+    ps = two()
+    opt = cls(ps)
+
+    def halve(o):
+        for st in o.state.values():
+            st['exp_avg'].mul_(0.5)
+    opt.register_load_state_dict_post_hook(halve)
+    opt.load_state_dict(saved(0.5, 0.25))
+    assert float(opt.state[ps[0]]['exp_avg'][0]) == 0.25 and float(opt.state[ps[1]]['exp_avg'][0]) == 0.125
