@@ -32,6 +32,10 @@ def own_max_norm(optimizer):
     return optimizer.max_norm if isinstance(optimizer, AdamW) else None
 
 
+# What torch.optim.AdamW keeps in its groups and has no say here.
+_OTHER_SETTINGS = ('amsgrad', 'maximize', 'foreach', 'differentiable', 'fused', 'decoupled_weight_decay')
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay; arguments as torch.optim.AdamW's, and
 
@@ -100,14 +104,15 @@ class AdamW(torch.optim.Optimizer):
             saved = state_dict['state'].get(i)
             if not saved:
                 continue
-            st = {k: torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(saved[k])
-                  for k in ('exp_avg', 'exp_avg_sq', 'master') if k in saved}
-            st['step'] = torch.as_tensor(saved['step'], dtype=torch.float32).to(p.device, copy=True).reshape(())
-            self.state[p] = st
-        for g in self.param_groups:
-            for k in list(g):
-                if k not in self.defaults and k not in ('params', 'initial_lr', 'param_names'):
-                    del g[k]
+            st = self.state[p]                  # (entries of other names stay as the base class loads them)
+            for k in ('exp_avg', 'exp_avg_sq', 'master'):
+                if k in saved:
+                    st[k] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(saved[k])
+            if 'step' in saved:
+                st['step'] = torch.as_tensor(saved['step'], dtype=torch.float32).to(p.device, copy=True).reshape(())
+        for g in self.param_groups:             # (a scheduler's or a user's own options of a group stay)
+            for k in _OTHER_SETTINGS:
+                g.pop(k, None)
             g['capturable'] = True
 
     def _init_state(self, params):

@@ -1,4 +1,4 @@
-"""Loading the AdamW step's state (no GPU needed)."""
+"""Loading the AdamW step's state: hooks, the groups' own options, extra entries (no GPU needed)."""
 import pytest
 import torch
 
@@ -68,3 +68,40 @@ def test_a_post_hook_has_the_last_word(cls):
     opt.register_load_state_dict_post_hook(halve)
     opt.load_state_dict(saved(0.5, 0.25))
     assert float(opt.state[ps[0]]['exp_avg'][0]) == 0.25 and float(opt.state[ps[1]]['exp_avg'][0]) == 0.125
+
+
+@pytest.mark.parametrize('cls', [optim.AdamW, torch.optim.AdamW])
+def test_a_scheduler_goes_on_after_loading(cls):
+    ps = two()
+    opt = cls(ps, lr=0.1)
+    sched = torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=0.1, total_steps=10)
+    opt.load_state_dict(opt.state_dict())
+    was = opt.param_groups[0]['lr']
+    opt._opt_called = True                  # (no step was taken: there is no device here)
+    sched.step()
+    assert opt.param_groups[0]['lr'] != was and opt.param_groups[0]['max_lr'] == 0.1
+
+
+def test_a_groups_own_options_are_kept_and_the_other_optimizers_settings_are_not():
+    ps = two()
+    groups = [dict(params=[ps[0]], name='trunk', lr_scale=0.5), dict(params=[ps[1]], name='heads')]
+    opt = optim.AdamW(groups)
+    opt.load_state_dict(opt.state_dict())
+    assert opt.param_groups[0]['name'] == 'trunk' and opt.param_groups[0]['lr_scale'] == 0.5
+    assert opt.param_groups[1]['name'] == 'heads' and 'lr_scale' not in opt.param_groups[1]
+    other = torch.optim.AdamW([dict(params=[ps[0]], name='a'), dict(params=[ps[1]], name='b')], foreach=True)
+    opt.load_state_dict(other.state_dict())
+    for g, name in zip(opt.param_groups, 'ab'):
+        assert g['name'] == name and g['capturable'] is True
+        assert not {'foreach', 'fused', 'amsgrad', 'maximize', 'differentiable', 'decoupled_weight_decay'} & set(g)
+
+
+def test_extra_entries_of_a_state_are_kept():
+    ps = two()
+    opt = optim.AdamW(ps)
+    state = saved(0.1, 0.2)
+    state['state'][0]['seen'] = 7
+    state['state'][0]['trace'] = torch.arange(4.0)
+    opt.load_state_dict(state)
+    assert opt.state[ps[0]]['seen'] == 7 and torch.equal(opt.state[ps[0]]['trace'], torch.arange(4.0))
+    assert 'seen' not in opt.state[ps[1]]
