@@ -36,8 +36,16 @@ def own_max_norm(optimizer):
 _OTHER_SETTINGS = ('amsgrad', 'maximize', 'foreach', 'differentiable', 'fused', 'decoupled_weight_decay')
 
 
+def _refuse_settings(settings):
+    for k in ('amsgrad', 'maximize', 'differentiable'):
+        if settings.get(k):
+            raise ValueError(f'AdamW: {k} is not supported')
+
+
 class AdamW(torch.optim.Optimizer):
-    """AdamW with decoupled weight decay; arguments as torch.optim.AdamW's, and
+    """AdamW with decoupled weight decay; arguments as torch.optim.AdamW's (`foreach`, `fused` and `capturable` choose among
+    its ways to the same result and change nothing here; `amsgrad`, `maximize` and `differentiable` are refused where they
+    are true), and, as the sixth to eighth,
 
     max_norm         the gradients are scaled by min(1, max_norm / (norm + 1e-6)) as they are read (`.grad` itself is not
                      written); the norm is taken over all parameter groups together.  None: no clipping.
@@ -54,7 +62,11 @@ class AdamW(torch.optim.Optimizer):
     which a replay reads afresh.  The state is laid out by the first step, which therefore cannot be a captured one."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, norm_type=2.0,
-                 skip_nonfinite=False):
+                 skip_nonfinite=False, *, amsgrad=False, maximize=False, foreach=None, capturable=True, differentiable=False,
+                 fused=None):
+        _refuse_settings(dict(amsgrad=amsgrad, maximize=maximize, differentiable=differentiable))
+        if isinstance(max_norm, bool):          # (torch.optim.AdamW's sixth argument is amsgrad)
+            raise ValueError(f'max_norm must be a number or None, got {max_norm}')
         if not torch.is_tensor(lr) and not lr >= 0.0:
             raise ValueError(f'invalid learning rate: {lr}')
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
@@ -68,6 +80,11 @@ class AdamW(torch.optim.Optimizer):
         self.norm_type, self.skip_nonfinite = float(norm_type), bool(skip_nonfinite)
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, capturable=True))
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):       # (the base class says what else it takes)
+            _refuse_settings(param_group)
+        super().add_param_group(param_group)
 
     def __getstate__(self):         # (copies and pickles: the base class names what it keeps)
         return dict(super().__getstate__(), max_norm=self.max_norm, norm_type=self.norm_type,
@@ -85,8 +102,7 @@ class AdamW(torch.optim.Optimizer):
 
         def check_loaded(_, sd):                # behind the other pre-hooks, each of which may put another dict in its place
             for g in sd['param_groups']:
-                if g.get('amsgrad') or g.get('maximize'):
-                    raise ValueError('AdamW: amsgrad and maximize are not supported')
+                _refuse_settings(dict(g, differentiable=False))
             loaded.update(sd)
         hooks = (self.register_load_state_dict_pre_hook(check_loaded),
                  self.register_load_state_dict_post_hook(lambda _: self._lay_out(loaded), prepend=True))

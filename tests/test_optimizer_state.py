@@ -1,4 +1,5 @@
-"""Loading the AdamW step's state: hooks, the groups' own options, extra entries (no GPU needed)."""
+"""Loading the AdamW step's state: hooks, the groups' own options, extra entries, and the settings that it accepts (no GPU
+needed)."""
 import pytest
 import torch
 
@@ -105,3 +106,23 @@ def test_extra_entries_of_a_state_are_kept():
     opt.load_state_dict(state)
     assert opt.state[ps[0]]['seen'] == 7 and torch.equal(opt.state[ps[0]]['trace'], torch.arange(4.0))
     assert 'seen' not in opt.state[ps[1]]
+
+
+def test_settings_of_the_other_optimizer():
+    """What asks for nothing, or for one of the other optimizer's ways to the same result, is taken; the rest is refused."""
+    for kw in (dict(amsgrad=False), dict(maximize=False), dict(differentiable=False), dict(foreach=False), dict(foreach=True),
+               dict(foreach=None), dict(fused=True), dict(fused=False), dict(capturable=False), dict(capturable=True)):
+        opt = optim.AdamW(two(), lr=0.5, **kw)
+        assert opt.param_groups[0]['lr'] == 0.5 and opt.param_groups[0]['capturable'] is True and opt.max_norm is None
+    for kw in (dict(amsgrad=True), dict(maximize=True), dict(differentiable=True)):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            optim.AdamW(two(), **kw)
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            optim.AdamW([dict(params=two(), **kw)])
+
+
+@pytest.mark.parametrize('value', [True, False])
+def test_a_truth_value_is_no_max_norm(value):
+    """The other optimizer's sixth argument is amsgrad: in its place here stands a number."""
+    with pytest.raises(ValueError, match='max_norm'):
+        optim.AdamW(two(), 1e-3, (0.9, 0.999), 1e-8, 0.01, value)
