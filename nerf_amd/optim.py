@@ -52,8 +52,9 @@ class AdamW(torch.optim.Optimizer):
     norm_type        2, 1 or inf.
     skip_nonfinite   a step whose gradient norm is infinite or NaN leaves parameters, moments and step counters as they are.
 
-    `grad_norm` holds the norm of the last step (a 0-d fp32 tensor on the device, which the replays of a captured step
-    write again; None before the first, and without max_norm or skip_nonfinite).
+    `grad_norm` holds the norm of the last step, replays of captured ones included (a 0-d fp32 tensor on the device; None
+    before the first step, and without max_norm or skip_nonfinite).  Each step has a tensor of its own until one is captured:
+    from then on it is one tensor, which every later step and every replay write, so that what is to be kept is cloned.
 
     Parameters are fp32, bf16 or fp16, on one HIP device, their gradients of the same type.  The moments are fp32 whatever
     the parameters are, and a 16-bit parameter has an fp32 master weight in the state ('master'), of which it is the
@@ -78,7 +79,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm = None if max_norm is None else ops.check_max_norm(max_norm)
         self._kind = ops.norm_kind(norm_type)
         self.norm_type, self.skip_nonfinite = float(norm_type), bool(skip_nonfinite)
-        self.grad_norm = None
+        self.grad_norm = self._graph_norm = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, capturable=True))
 
     def add_param_group(self, param_group):
@@ -88,7 +89,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __getstate__(self):         # (copies and pickles: the base class names what it keeps)
         return dict(super().__getstate__(), max_norm=self.max_norm, norm_type=self.norm_type,
-                    skip_nonfinite=self.skip_nonfinite, _kind=self._kind, grad_norm=None)
+                    skip_nonfinite=self.skip_nonfinite, _kind=self._kind, grad_norm=None, _graph_norm=None)
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -162,7 +163,8 @@ class AdamW(torch.optim.Optimizer):
             ops.list_call(device, lambda st: self._launch(device, len(params), memoryview(counts).cast('i'), arrays, st))
             torch.autograd.graph.increment_version(params)      # (the kernels write behind autograd's back)
         elif self.max_norm is not None or self.skip_nonfinite:
-            self.grad_norm = torch.zeros((), device=next((p.device for ps in lists_of for p in ps), None))
+            self.grad_norm = (torch.zeros((), device=next((p.device for ps in lists_of for p in ps), None))
+                              if self._graph_norm is None else self._graph_norm.zero_())
         return loss
 
     def _launch(self, device, n, counts, arrays, st):
@@ -187,7 +189,13 @@ class AdamW(torch.optim.Optimizer):
         clips = self.max_norm is not None or self.skip_nonfinite
         nbytes = L.nerf_grad_workspace_bytes(n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device='cuda')
-        norm = torch.empty((), dtype=torch.float32, device='cuda') if clips else None
+        norm = None
+        if clips:       # (a replay runs no Python: what it writes has to be what grad_norm names whichever step ran before it)
+            norm = self._graph_norm
+            if norm is None or norm.get_device() != device:
+                norm = torch.empty((), dtype=torch.float32, device='cuda')
+                if torch.cuda.is_current_stream_capturing():
+                    self._graph_norm = norm
         check(L.nerf_adamw_step(ctypes.byref(AdamwTensors(n, *arrays)), groups, len(counts), self._kind if clips else 0,
                                 float('inf') if self.max_norm is None else self.max_norm, int(self.skip_nonfinite),
                                 ws.data_ptr(), nbytes, norm.data_ptr() if clips else None, st))
