@@ -207,11 +207,26 @@ __device__ __forceinline__ double norm_of(const Clip& c) {
     return norm_of<NERF_NORM_MAX>(c.partials, c.n_partials);
 }
 
-// Formed in 64 bits, rounded once to the 32 bits that the entries are multiplied in.
-__device__ __forceinline__ float coefficient(double norm, double max_norm) {
+// factor * 2^exponent: formed in 64 bits, the factor rounded once to the 32 bits that the entries are multiplied in.  The
+// exponent is 0 but for a coefficient below fp32's normal range, which would keep few bits there, or none: the entries
+// that bring such a norm about are so large that their products are ordinary numbers again.
+struct Scale {
+    float factor = 1.f;
+    int exponent = 0;
+};
+
+__device__ __forceinline__ Scale coefficient(double norm, double max_norm) {
+    Scale s;
     const double d = norm + 1e-6;
-    return d <= max_norm ? 1.f : (float)(max_norm / d);       // (a NaN norm gives NaN)
+    if (d <= max_norm) return s;
+    double c = max_norm / d;                                // (a NaN norm gives NaN)
+    if (c > 0.0 && c < 0x1p-126) c = frexp(c, &s.exponent);
+    s.factor = (float)c;
+    return s;
 }
+
+// One product in 32 bits; the power of two is exact, but for results below the normal range, and one instruction.
+__device__ __forceinline__ float scaled(float x, const Scale& s) { return ldexpf(x * s.factor, s.exponent); }
 
 // Bound by reading: 4.3 GB fp32 in one tensor 615 us, 7.0 TB/s; 6e8 bytes of bf16 in 389 tensors 107 us (two launches),
 // 5.6 TB/s.  The 64-bit multiply-adds (one per element, half the fp32 rate) are a tenth of that.
@@ -274,7 +289,7 @@ __global__ __launch_bounds__(kThreads) void scale_by_norm(ListTable tab, Clip cl
     using P = Pack<T, V, STREAM>;
     const double norm = norm_of(clip);
     if (blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = (float)norm;
-    const float s = coefficient(norm, clip.max_norm);
+    const Scale s = coefficient(norm, clip.max_norm);
     const int total = tab.end[tab.n - 1];
     Cursor<ListTable::kCap> c(tab);
     T* g = nullptr;
@@ -288,10 +303,10 @@ __global__ __launch_bounds__(kThreads) void scale_by_norm(ListTable tab, Clip cl
             if (i >= 0 && i + V <= c.hi) {
                 typename P::type x = P::load(g + i);
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[j] = (T)((float)x[j] * s);
+                for (int j = 0; j < V; ++j) x[j] = (T)scaled((float)x[j], s);
                 P::store(g + i, x);
             } else {
-                for (int64_t j = i < 0 ? 0 : i; j < i + V && j < c.hi; ++j) g[j] = (T)((float)g[j] * s);
+                for (int64_t j = i < 0 ? 0 : i; j < i + V && j < c.hi; ++j) g[j] = (T)scaled((float)g[j], s);
             }
         }
     }
@@ -302,12 +317,13 @@ __device__ __forceinline__ float of_lane(float x, int lane) {
 }
 
 struct Factors {
-    float clip, lr, inv1, inv2;     // inv1 = 1 / (1 - beta1^t), inv2 = 1 / sqrt(1 - beta2^t)
+    Scale clip;
+    float lr, inv1, inv2;           // inv1 = 1 / (1 - beta1^t), inv2 = 1 / sqrt(1 - beta2^t)
 };
 
 // One entry: its weight in 32 bits (the parameter itself, or its master), gradient and moments.
 __device__ __forceinline__ void adamw_entry(float& w, float g, float& m, float& v, const AdamArgs& a, const Factors& f) {
-    g *= f.clip;
+    g = scaled(g, f.clip);
     m = a.beta1 * m + a.rest1 * g;
     v = a.beta2 * v + a.rest2 * (g * g);
     w -= f.lr * (m * f.inv1 / (sqrtf(v) * f.inv2 + a.eps) + a.decay * w);
@@ -335,7 +351,6 @@ __global__ __launch_bounds__(kThreads) void adamw(AdamTable tab, Clip clip, Adam
     using P = Pack<T, V, STREAM>;
     using F = Pack<float, V, STREAM>;
     Factors f;
-    f.clip = 1.f;
     if (clip.partials) {
         const double norm = norm_of(clip);
         if (blockIdx.x == 0 && threadIdx.x == 0 && clip.norm) *clip.norm = (float)norm;

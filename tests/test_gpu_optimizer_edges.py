@@ -1,11 +1,55 @@
-"""Corners of the gradient norm, clipping and the AdamW step that need a device: the norm that an optimizer shows.
-Tolerances as counted in test_gpu_optimizer."""
+"""Corners of the gradient norm, clipping and the AdamW step that need a device: coefficients below fp32's normal range,
+the norm that an optimizer shows.  Tolerances as counted in test_gpu_optimizer."""
 import pytest
 import torch
 
-from tests.test_gpu_optimizer import (SIZES, gen, near_norm, norm64, params_of)
+from tests.test_gpu_optimizer import (DTYPES, HALF_STEP, NORMS, SIZES, TINY, U, check_step, gen, make, make_state,
+                                      near_norm, norm64, optimizer, params_of, snapshot)
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- coefficients below the normal range of fp32 ------------------------------------------------------------------
+
+def huge(dtype, n=4099):
+    """Entries of the size of the type's largest; their norm is beyond fp32 (but for fp16)."""
+    x = torch.rand(n, device='cuda', generator=gen(9)) * 0.5 + 0.5
+    x[::3] *= -1
+    return (x.double() * 0.99 * torch.finfo(dtype).max).to(dtype)
+
+
+# the coefficient itself: normal, on both sides of 2^-126, subnormal, below the smallest subnormal, and far below
+COEFFICIENTS = [2.0 ** -100, 2.0 ** -126 * (1 + 2.0 ** -10), 2.0 ** -126 * (1 - 2.0 ** -10), 2.0 ** -133, 1.1e-43, 2.0 ** -151,
+                3e-48, 1e-60, 1e-200]
+
+
+@pytest.mark.parametrize('coefficient', COEFFICIENTS)
+@pytest.mark.parametrize('norm_type', NORMS)
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_clip_by_a_coefficient_below_the_normal_range(dtype, norm_type, coefficient):
+    from nerf_amd import ops
+    t = huge(dtype)
+    was, norm = t.double(), norm64([t], norm_type)
+    got = ops.clip_grad_norm_(t, coefficient * norm, norm_type)
+    assert float(got) == float(torch.tensor(norm, dtype=torch.float64).float())
+    want = was * (coefficient * norm / (norm + 1e-6))
+    # the coefficient, the product, the rounding to the type; below the normal ranges half a smallest step of both types
+    tol = want.abs() * (2 * U + HALF_STEP[dtype]) * (1 + U) + TINY[dtype] + 2.0 ** -150
+    off = (t.double() - want).abs() - tol
+    assert bool((off <= 0).all()), float(off.max())
+
+
+@pytest.mark.parametrize('coefficient', COEFFICIENTS)
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_adamw_with_a_coefficient_below_the_normal_range(dtype, coefficient):
+    p = torch.nn.Parameter(make([4099], dtype, scale=0.3)[0].clone())
+    p.grad = huge(dtype)
+    norm = norm64([p.grad], 2.0)
+    states = make_state([p], 0)             # (moments of zero: what the gradient adds is all there is)
+    was = snapshot([p], states)
+    opt = optimizer([p], states, max_norm=coefficient * norm)
+    opt.step()
+    check_step([p], was, states, 1, coefficient * norm / (norm + 1e-6))
 
 
 # ---- the norm that an optimizer shows -----------------------------------------------------------------------------
