@@ -429,7 +429,8 @@ int nerf_clip_grad_norm(void* const* grads, const int64_t* numel, const int32_t*
  * master restarts from the parameter.  `dtype` is that of the parameter and of its gradient.  skip_nonfinite != 0 (with a
  * norm): where the norm is infinite or NaN nothing but `norm` is written.  groups[k] holds the settings of the next
  * `count` parameters of the list; lr_device (nullable) is an fp32 learning rate on the device, read in place of `lr`.
- * norm[1] (nullable) receives the norm before clipping, over all groups.  Parameters must not share memory. */
+ * norm[1] (nullable) receives the norm before clipping, over all groups (0 for an empty list, which needs no workspace).
+ * Neither the parameters nor what is kept for them may share memory. */
 typedef struct nerf_adamw_tensors {
     int n_tensors;
     void* const* param;

@@ -632,7 +632,11 @@ extern "C" int nerf_adamw_step(const nerf_adamw_tensors* t, const nerf_adamw_gro
     const bool clips = norm_kind != NERF_NORM_NONE;
     NERF_REQUIRE(!clips || (known_kind(norm_kind) && max_norm >= 0.0));
     NERF_REQUIRE(clips || !skip_nonfinite);
-    if (n == 0) return NERF_OK;
+    if (n == 0) {
+        if (!clips || !norm) return NERF_OK;
+        norm_finish<<<1, kThreads, 0, nerf_stream(stream)>>>(Clip{nullptr, 0, norm_kind, 0, 0.0, norm});
+        return nerf_launch_status();
+    }
     Workspace ws;
     if (int e = take_workspace(workspace, n_workspace, n, &ws)) return e;
     if (int e = check_disjoint(t->param, t->numel, t->dtype, n)) return e;

@@ -1,5 +1,7 @@
 """Corners of the gradient norm, clipping and the AdamW step that need a device: coefficients below fp32's normal range,
-the norm that an optimizer shows.  Tolerances as counted in test_gpu_optimizer."""
+the norm that an optimizer shows, empty lists at the C entry.  Tolerances as counted in test_gpu_optimizer."""
+import ctypes
+
 import pytest
 import torch
 
@@ -82,3 +84,17 @@ def test_grad_norm_after_eager_and_captured_steps():
         p.grad = None
     opt.step()
     assert float(opt.grad_norm) == 0
+
+
+# ---- the C entry with nothing to update ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize('kind', [1, 2, 3])
+def test_c_adamw_of_an_empty_list_writes_the_norm(kind):
+    from nerf_amd import _lib
+    L = _lib.lib()
+    norm = torch.full((3,), 5.0, device='cuda')
+    torch.cuda.synchronize()
+    t = _lib.AdamwTensors(0, *([None] * 8))
+    assert L.nerf_adamw_step(ctypes.byref(t), None, 0, kind, 1.0, 0, None, 0, norm[1:].data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    assert norm.tolist() == [5.0, 0.0, 5.0]
