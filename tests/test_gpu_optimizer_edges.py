@@ -1,12 +1,14 @@
 """Corners of the gradient norm, clipping and the AdamW step that need a device: coefficients below fp32's normal range,
-the norm that an optimizer shows, empty lists at the C entry.  Tolerances as counted in test_gpu_optimizer."""
+the norm that an optimizer shows, empty lists at the C entry, inference mode, refused gradients, state at odd places,
+lists past the caches.  Tolerances as counted in test_gpu_optimizer."""
 import ctypes
+import math
 
 import pytest
 import torch
 
-from tests.test_gpu_optimizer import (DTYPES, HALF_STEP, NORMS, SIZES, TINY, U, check_step, gen, make, make_state,
-                                      near_norm, norm64, optimizer, params_of, snapshot)
+from tests.test_gpu_optimizer import (DTYPES, HALF_STEP, NORMS, SIZES, TINY, U, check_clipped, check_step, gen, make,
+                                      make_state, near_norm, norm64, optimizer, params_of, snapshot)
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +100,139 @@ def test_c_adamw_of_an_empty_list_writes_the_norm(kind):
     assert L.nerf_adamw_step(ctypes.byref(t), None, 0, kind, 1.0, 0, None, 0, norm[1:].data_ptr(), None) == 0
     torch.cuda.synchronize()
     assert norm.tolist() == [5.0, 0.0, 5.0]
+
+
+# ---- inference mode -----------------------------------------------------------------------------------------------
+
+def test_tensors_of_inference_mode():
+    from nerf_amd import ops, optim
+    plain = make([300, 40], torch.float32)
+    version = plain[1]._version
+    was = [t.double() for t in plain]
+    with torch.inference_mode():
+        ts = [t.clone() for t in plain]
+        check_clipped(ts, was, 0.01, 2.0, ops.clip_grad_norm_(ts, 0.01))
+        mixed = [ts[0].copy_(plain[0]), plain[1]]
+        check_clipped(mixed, was, 0.01, 2.0, ops.clip_grad_norm_(mixed, 0.01))
+        near_norm(ops.grad_norm(ts), norm64(ts, 2.0))
+        p = torch.nn.Parameter(torch.ones(500, device='cuda'))
+        p.grad = torch.ones(500, device='cuda')
+        opt = optim.AdamW([p], lr=0.25, weight_decay=0.0)
+        opt.step()
+        assert torch.allclose(p, torch.full_like(p, 0.75), rtol=0, atol=1e-6)
+    assert plain[1]._version > version
+
+
+# ---- gradients that are refused stay as they were -----------------------------------------------------------------
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('bad', [math.nan, -math.nan, math.inf, -math.inf])
+def test_refused_gradients_keep_their_bits(dtype, bad):
+    from nerf_amd import optim
+    ps = params_of([700, 5001, 3], dtype)
+    ps[1].grad[2500] = bad
+    bits = lambda t: t.detach().clone().view(torch.int32 if dtype == torch.float32 else torch.int16)     # noqa: E731
+    was = [bits(p.grad) for p in ps]
+    with pytest.raises(RuntimeError, match='not finite'):
+        optim.clip_grad_norm_(ps, 1e-3, error_if_nonfinite=True)
+    assert all(torch.equal(bits(p.grad), w) for p, w in zip(ps, was))
+
+
+# ---- state at odd places ------------------------------------------------------------------------------------------
+
+def guarded(values, offset):
+    """A copy of `values` that starts `offset` elements into a buffer of 77s."""
+    n = values.numel()
+    buf = torch.full((offset + n + 40,), 77.0, device='cuda', dtype=values.dtype)
+    buf[offset:offset + n] = values
+    return buf[offset:offset + n]
+
+
+def guards_kept(view, offset):
+    whole = torch.as_strided(view, (offset + view.numel() + 40,), (1,), 0)
+    assert bool((whole[:offset] == 77).all()) and bool((whole[offset + view.numel():] == 77).all())
+
+
+# elements ahead of exp_avg, exp_avg_sq, master, parameter and gradient in their buffers (a line of memory holds 32 fp32)
+PLACES = [(1, 0, 0, 0, 0), (3, 3, 3, 3, 3), (31, 1, 2, 3, 5), (5, 33, 30, 1, 7), (32, 31, 6, 9, 2), (30, 17, 13, 63, 1)]
+
+
+@pytest.mark.parametrize('clip', [None, 2.0])
+@pytest.mark.parametrize('places', PLACES)
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_adamw_with_state_at_odd_places(dtype, places, clip):
+    sizes = [1, 2, 3, 4, 5, 30, 31, 33, 0, 1023, 1024, 1025, 2048 - places[0], 2049 - places[0], 70_001]
+    ps, states = [], []
+    for p, st in zip(params_of(sizes, dtype), make_state(params_of(sizes, dtype), 10)):
+        q = torch.nn.Parameter(guarded(p.detach(), places[3]))
+        q.grad = guarded(p.grad, places[4])
+        st.update(exp_avg=guarded(st['exp_avg'], places[0]), exp_avg_sq=guarded(st['exp_avg_sq'], places[1]))
+        if dtype != torch.float32:
+            st['master'] = guarded(p.detach().float(), places[2])
+        ps.append(q)
+        states.append(st)
+    was = snapshot(ps, states)
+    n = norm64([p.grad for p in ps], 2.0)
+    opt = optimizer(ps, states, max_norm=0.4 * n if clip else None)
+    opt.step()
+    check_step(ps, was, states, 11, 0.4 * n / (n + 1e-6) if clip else 1.0)
+    for p, st in zip(ps, states):
+        for view, offset in zip((st['exp_avg'], st['exp_avg_sq'], st.get('master'), p.data, p.grad), places):
+            if view is not None:
+                guards_kept(view, offset)
+
+
+# ---- lists past the caches ----------------------------------------------------------------------------------------
+
+def packed(total, dtype, seed, first=1):
+    """Seven ragged tensors of `total` elements, behind one another from an odd place of one buffer on."""
+    parts = [total // 3 + 1, 5, total // 4 + 3, 1, 0, total // 5]
+    sizes = parts + [total - sum(parts)]
+    flat = torch.full((first + total + 40,), 77.0, device='cuda', dtype=dtype)
+    flat[first:first + total] = 0.01 * torch.randn(total, device='cuda', generator=gen(seed))
+    out, at = [], first
+    for k, n in enumerate(sizes):
+        out.append(flat[at:at + n])
+        out[-1].mul_(1 + k)
+        at += n
+    return flat, out
+
+
+def ends_kept(flat, total, first=1):
+    assert bool((flat[:first] == 77).all()) and bool((flat[first + total:] == 77).all())
+
+
+@pytest.mark.parametrize('norm_type', NORMS)
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_norm_and_clip_of_lists_past_the_caches(dtype, norm_type):
+    from nerf_amd import ops
+    total = (30_000_001 if dtype == torch.float32 else 60_000_001)      # 120 MB to read, 240 MB to read and write
+    flat, ts = packed(total, dtype, seed=4)
+    near_norm(ops.grad_norm(ts, norm_type), norm64(ts, norm_type))
+    was = [t.double() for t in ts]
+    most = 0.3 * norm64(ts, norm_type)
+    check_clipped(ts, was, most, norm_type, ops.clip_grad_norm_(ts, most, norm_type))
+    ends_kept(flat, total)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_adamw_of_lists_past_the_caches(dtype):
+    total = 9_000_001               # 252 MB and more
+    flats, lists = zip(*[packed(total, d, seed=k, first=f) for k, (d, f) in
+                         enumerate([(dtype, 1), (dtype, 3), (torch.float32, 5), (torch.float32, 2), (torch.float32, 7)])])
+    ps, states = [], []
+    for p, g, m, v, w in zip(*lists):
+        v.abs_().mul_(1e-2)
+        ps.append(torch.nn.Parameter(p))
+        ps[-1].grad = g
+        states.append(dict(step=torch.tensor(10.0, device='cuda'), exp_avg=m, exp_avg_sq=v))
+        if dtype != torch.float32:
+            states[-1]['master'] = w.copy_(p)
+    was = snapshot(ps, states)
+    n = norm64([p.grad for p in ps], 2.0)
+    opt = optimizer(ps, states, max_norm=0.4 * n)
+    opt.step()
+    near_norm(opt.grad_norm, n)
+    check_step(ps, was, states, 11, 0.4 * n / (n + 1e-6))
+    for flat, first in zip(flats, (1, 3, 5, 2, 7)):
+        ends_kept(flat, total, first)
