@@ -6,6 +6,8 @@ call raises.
 """
 import ctypes
 import os
+import re
+import sys
 from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
@@ -128,6 +130,10 @@ def lists():
             from . import _tensor_lists
         except ImportError as e:
             raise ImportError(f'nerf_amd._tensor_lists: {e} (build it with `python -m nerf_amd.build`)') from None
+        here = (re.match(r'[\d.]*\d', torch.__version__).group(), '%d.%d' % sys.version_info[:2])
+        if getattr(_tensor_lists, 'built_for', None) != here:
+            raise ImportError('nerf_amd._tensor_lists was built for another torch or Python than %s, %s (build it again with '
+                              '`python -m nerf_amd.build`)' % here)
         _lists = _tensor_lists
     return _lists
 

@@ -39,6 +39,7 @@ UNITS = {
 UNITS.update({'mlp_bf16_p%d.o' % p: ('mlp_bf16.hip', ['-DNERF_NET_PART=%d' % p]) for p in range(8)})   # default contraction
 LISTS_SRC = os.path.join(CSRC, 'tensor_lists.cpp')
 LISTS = os.path.join(HERE, '_tensor_lists.so')
+LISTS_RECORD = os.path.join(OBJDIR, 'tensor_lists.txt')         # what LISTS was built with
 JOBS = int(os.environ.get('MAX_JOBS', '8'))
 
 
@@ -68,6 +69,19 @@ def _lists_command():
             + [LISTS_SRC, '-o', LISTS, '-L' + libdir, '-ltorch_python', '-ltorch_cpu', '-lc10'])
 
 
+def lists_record():
+    """The host module goes by torch's C++ headers and by Python's: its command and both versions."""
+    import torch
+    return '\n'.join([' '.join(_lists_command()), torch.__version__, sys.version])
+
+
+def lists_stale():
+    if _stale(LISTS, [LISTS_SRC, os.path.abspath(__file__)]) or not os.path.exists(LISTS_RECORD):
+        return True
+    with open(LISTS_RECORD) as f:
+        return f.read() != lists_record()
+
+
 def build(force=False, verbose=True):
     os.makedirs(OBJDIR, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(('.h', '.inc'))]
@@ -80,7 +94,7 @@ def build(force=False, verbose=True):
         objs.append(obj)
         if force or _stale(obj, [src] + headers):
             jobs.append([_hipcc()] + COMMON + extra + ['-c', src, '-o', obj])
-    host = [_lists_command()] if force or _stale(LISTS, [LISTS_SRC, os.path.abspath(__file__)]) else []
+    host = [_lists_command()] if force or lists_stale() else []
     for f in os.listdir(OBJDIR):                      # objects of an older unit list must not be linked
         if f.endswith('.o') and f not in UNITS:
             os.remove(os.path.join(OBJDIR, f))
@@ -92,6 +106,9 @@ def build(force=False, verbose=True):
 
     with ThreadPoolExecutor(max_workers=min(JOBS, max(1, len(jobs + host)))) as ex:
         list(ex.map(run, jobs + host))
+    if host:
+        with open(LISTS_RECORD, 'w') as f:
+            f.write(lists_record())
     if jobs or force or _stale(LIB, objs):
         run([_hipcc(), '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB] + objs)
     return LIB

@@ -12,12 +12,14 @@
 //                                number per group and the nerf_adamw_tensors arrays param, grad, exp_avg, exp_avg_sq,
 //                                master, step, numel, dtype)
 //   is_dense(tensor)          -> bool
+//   built_for                    versions of torch and Python whose headers the module was built with
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <vector>
 
@@ -246,4 +248,14 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_lists", nullptr, -1, metho
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tensor_lists() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__tensor_lists() {
+    PyObject* m = PyModule_Create(&module);
+    if (!m) return nullptr;
+    PyObject* v = Py_BuildValue("(sN)", TORCH_VERSION, PyUnicode_FromFormat("%d.%d", PY_MAJOR_VERSION, PY_MINOR_VERSION));
+    if (!v || PyModule_AddObject(m, "built_for", v)) {
+        Py_XDECREF(v);
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}
