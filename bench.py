@@ -55,7 +55,7 @@ def make_cfg(precision='bf16'):
                            mlp_precision=precision)
 
 
-PMC_TRAFFIC = 'r03_pmc_traffic.json'
+PMC_TRAFFIC = 'pmc_traffic.json'
 KERNEL_SOURCES = ('nerf_amd/csrc', 'nerf_amd/stepper.py', 'nerf_amd/mlp_bf16.py')
 
 

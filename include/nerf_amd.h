@@ -393,7 +393,8 @@ int nerf_mlp_wgrad8_config(int n_feat0, int n_feat1, int k_feat0, int k_feat1, i
  * element order does not matter, and they may start at any multiple of their element size.  The arrays are read before
  * the call returns.  `workspace`: nerf_grad_workspace_bytes(n_tensors) bytes of device scratch, 8-byte aligned, whose
  * contents mean nothing between calls; calls that may overlap on the device each need their own.  Sums and norms are held
- * in 64 bits and added in a fixed order: the same bits on every call, and no overflow or underflow of the squares.
+ * in 64 bits, with no overflow or underflow of the squares, and added in an order that goes by the list and by where its
+ * tensors start within their 128-byte lines of memory: the same bits wherever these are alike, as on the ranks of a job.
  *                              reference: torch.optim.AdamW (model.py:177-181); it has no clipping */
 #define NERF_F32 0
 #define NERF_BF16 1

@@ -11,7 +11,8 @@
 // several launches.  Each tensor is cut into chunks, which the workgroups of a launch take in turn, so that all of them
 // together sweep through memory.  The norm is one launch that leaves a partial sum per workgroup in the caller's
 // workspace; every workgroup of the launch that needs the norm adds those up for itself, in one fixed order, so that
-// there are no atomics, no waiting between workgroups, no launch in between, and the same bits on every call.
+// there are no atomics, no waiting between workgroups and no launch in between.  The order of a sum goes by the list and
+// by where its tensors start within a line of memory: alike in these, two calls give the same bits.
 #include <stdlib.h>
 
 #include <algorithm>
@@ -26,11 +27,12 @@ constexpr int kThreads = 256;
 
 // How a kernel's launches are cut: at most `groups` workgroups, and chunks of `least` elements (one access per lane) while
 // the list is short, so that every compute unit gets some, up to `most` for a long one.  What the workgroups touch at one
-// time (groups x chunk, in each of the tensors' arrays) is kept to a few megabytes: AdamW over 1e8 fp32 parameters took
-// 702 us with 2048 workgroups and chunks of 16384, 604 with 1024 and 16384, 567 with 1024 and 4096, 547 with 768 and
-// 2048, 531 with 512 and 2048 (582 with 640, 588 with 256 and twice the loads under way); the norm of 4.3 GB 770 us with 2048 and 16384, 736
-// with 1024, the same at 1024 for chunks of 8192 to 32768; its inner loop wants four accesses per lane and chunk (5e8
-// bf16 elements in chunks of 4096: 190 us, of 16384: 128).
+// time (groups x chunk, in each of the tensors' arrays) is kept to a few megabytes: AdamW over 1e8 fp32 parameters in 128
+// tensors takes 618 us with 2048 workgroups and chunks of 16384, 578 with 1024 and 4096, 530 with 768 and 2048, 524 with
+// 512 and 2048 (551 with 512 and 4096, 536 with 512 and 1024, 580 with 640 and 2048, 608 with 256 and 2048); the norm of
+// 4.3 GB 628 us with 2048 and 16384, 616 with 2048 and 8192, 611 with 1024 and 4096 to 16384, 593 with 512 and 8192 (120 MB
+// 20.9 instead of 19.9).  Its inner loop wants four accesses per lane and chunk: with two 758 us, and 5e8 bf16 elements
+// 189 us instead of 147.
 struct Cut {
     int groups, least, most;
 };
@@ -40,10 +42,11 @@ constexpr Cut scale_cut(int size) { return {1024, 4096 / size, 16384 / size}; }
 constexpr Cut adam_cut(int) { return {512, 1024, 2048}; }
 
 // Accesses past the caches (non-temporal ones), in bytes of what a call reads and writes.  A norm that nothing follows:
-// 4.3 GB 613 us against 735 through the caches, 120 MB 25.1 against 28.4 and 40 MB 11.8 either way; 120 MB that were
-// written just before 61.5 against 62.7 (with the writing).  An update: AdamW of 280 MB 61.6 against 68.8, of 140 MB
-// 35.1 against 33.9.  The norm ahead of an update stays in the caches at any size: even where they hold only part of the
-// gradients the update finds some there (AdamW of 2.8 GB 546 us against 586, of 5.6 GB 1155 against 1183).
+// 4.3 GB 611 us against 690 through the caches, 120 MB 19.9 against 21.3 and 40 MB 11 either way; 120 MB that were
+// written just before 58.3 against 55.2 (with the writing).  An update with its norm: AdamW of 140 MB 33.8 against 31.8, of
+// 280 MB 58.1 against 54.6, of 2.8 GB 524 against 633, of 5.6 GB 1101 against 1246.  The norm ahead of an update stays
+// in the caches at any size: even where they hold only part of the gradients the update finds some there (AdamW of
+// 2.8 GB 524 us against 559, of 5.6 GB 1101 against 1126).
 constexpr int64_t kMiB = 1 << 20;
 constexpr int64_t kNormStream = 64 * kMiB;
 constexpr int64_t kUpdateStream = 192 * kMiB;
@@ -228,7 +231,7 @@ __device__ __forceinline__ Scale coefficient(double norm, double max_norm) {
 // One product in 32 bits; the power of two is exact, but for results below the normal range, and one instruction.
 __device__ __forceinline__ float scaled(float x, const Scale& s) { return ldexpf(x * s.factor, s.exponent); }
 
-// Bound by reading: 4.3 GB fp32 in one tensor 615 us, 7.0 TB/s; 6e8 bytes of bf16 in 389 tensors 107 us (two launches),
+// Bound by reading: 4.3 GB fp32 in one tensor 612 us, 7.0 TB/s; 6e8 bytes of bf16 in 389 tensors 107 us (two launches),
 // 5.6 TB/s.  The 64-bit multiply-adds (one per element, half the fp32 rate) are a tenth of that.
 template <typename T, int KIND, bool STREAM, typename Table>
 __global__ __launch_bounds__(kThreads) void norm_partials(Table tab, double* partials, float* steps) {
@@ -343,7 +346,8 @@ __device__ __forceinline__ void keep_rounded(float& x) { asm("" : "+v"(x)); }
 
 // Bound by memory: 28 bytes per fp32 parameter and 30 per 16-bit one; 1e8 fp32 parameters in 128 tensors 529 us with the
 // norm, 3.2 GB at 6.0 TB/s; 2.5e8 bf16 ones in 300 tensors 1400, 8.0 GB at 5.7 TB/s (three launches of the norm and six of
-// this, about 8 us each to drain and fill).  Division and square root are the correctly rounded ones; they hide behind the accesses.
+// this, about 8 us each to drain and fill).  Division and square root are the correctly rounded ones; they hide behind the
+// accesses.
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(kThreads) void adamw(AdamTable tab, Clip clip, AdamArgs a, const float* steps) {
     constexpr bool kMaster = sizeof(T) == 2;

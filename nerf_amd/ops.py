@@ -312,7 +312,8 @@ def _as_list(tensors):
 def grad_norm(tensors, norm_type=2.0):
     """The norm of all entries of a list of tensors (or of one tensor) together: `norm_type` 2, 1 or inf -> a 0-d fp32
     tensor on their device (no host synchronisation).  fp32, bf16 and fp16 tensors in one list as one likes; sums are held
-    in 64 bits and added in a fixed order.  A NaN entry gives NaN; an empty list gives 0.  No gradient flows through it."""
+    in 64 bits and added in a fixed order (of the list and of where its tensors start within their 128-byte lines).  A NaN
+    entry gives NaN; an empty list gives 0.  No gradient flows through it."""
     kind = norm_kind(norm_type)
     tensors = _as_list(tensors)
     table = _lib.lists().describe(tensors)

@@ -2,8 +2,10 @@
 backward pass and the next forward pass.
 
 `clip_grad_norm_` takes parameters and clips their gradients; `AdamW` is a `torch.optim.Optimizer` (learning-rate
-schedulers, parameter groups, `state_dict` as torch's own AdamW, model.py:177-181) whose step is two launches for all
-parameters together, takes the gradients' norm and clips them while it reads them, and can be captured into a HIP graph.
+schedulers, parameter groups, `state_dict` as torch's own AdamW, model.py:177-181) whose step takes the gradients' norm,
+clips them while it reads them, and can be captured into a HIP graph.  It is two launches for up to 56 parameters of one
+type in one group: the update is a launch per group, element type and 56 parameters, the norm ahead of it one
+per element type and 120 parameters (without a norm: one launch per 256 parameters, which copies the step counters).
 The tensor-level entry points are `nerf_amd.ops.grad_norm` and `nerf_amd.ops.clip_grad_norm_`.
 """
 import ctypes
@@ -50,7 +52,8 @@ class AdamW(torch.optim.Optimizer):
     max_norm         the gradients are scaled by min(1, max_norm / (norm + 1e-6)) as they are read (`.grad` itself is not
                      written); the norm is taken over all parameter groups together.  None: no clipping.
     norm_type        2, 1 or inf.
-    skip_nonfinite   a step whose gradient norm is infinite or NaN leaves parameters, moments and step counters as they are.
+    skip_nonfinite   a step whose gradient norm is infinite (in fp32) or NaN leaves parameters, moments and step counters as
+                     they are.
 
     `grad_norm` holds the norm of the last step, replays of captured ones included (a 0-d fp32 tensor on the device; None
     before the first step, and without max_norm or skip_nonfinite).  Each step has a tensor of its own until one is captured:
@@ -60,7 +63,8 @@ class AdamW(torch.optim.Optimizer):
     the parameters are, and a 16-bit parameter has an fp32 master weight in the state ('master'), of which it is the
     rounding; a parameter that something else writes is taken as it is, and its master follows.  The step counters live on
     the device, so a captured step counts on with every replay; the learning rate of a group may be an fp32 device tensor,
-    which a replay reads afresh.  The state is laid out by the first step, which therefore cannot be a captured one."""
+    which a replay reads afresh.  Gradients are taken as they are: where the loss was scaled (fp16), they are divided by the
+    scale ahead of the step.  The state is laid out by the first step, which therefore cannot be a captured one."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, norm_type=2.0,
                  skip_nonfinite=False, *, amsgrad=False, maximize=False, foreach=None, capturable=True, differentiable=False,
@@ -190,7 +194,7 @@ class AdamW(torch.optim.Optimizer):
         nbytes = L.nerf_grad_workspace_bytes(n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device='cuda')
         norm = None
-        if clips:       # (a replay runs no Python: what it writes has to be what grad_norm names whichever step ran before it)
+        if clips:       # (a replay runs no Python: what it writes has to be what grad_norm names, whatever ran before it)
             norm = self._graph_norm
             if norm is None or norm.get_device() != device:
                 norm = torch.empty((), dtype=torch.float32, device='cuda')

@@ -182,6 +182,21 @@ def test_adamw_with_state_at_odd_places(dtype, places, clip):
                 guards_kept(view, offset)
 
 
+@pytest.mark.parametrize('norm_type', NORMS)
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_the_same_bits_at_the_same_places_within_a_line(dtype, norm_type):
+    """Ranks hold their gradients at other addresses, but at the same places of their 128-byte lines: one norm, bit for bit."""
+    from nerf_amd import ops
+    values = make(SIZES['chunk'] + [70_001], dtype)
+    line = 128 // values[0].element_size()
+    for place in (0, 1, 5, line - 1):
+        got = []
+        for lines in (0, 1, 4, 33):
+            got.append(ops.grad_norm([guarded(v, place + lines * line) for v in values], norm_type))
+        near_norm(got[0], norm64(values, norm_type))
+        assert all(torch.equal(x, got[0]) for x in got)
+
+
 # ---- lists past the caches ----------------------------------------------------------------------------------------
 
 def packed(total, dtype, seed, first=1):
