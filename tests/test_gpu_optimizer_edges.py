@@ -1,14 +1,15 @@
 """Corners of the gradient norm, clipping and the AdamW step that need a device: coefficients below fp32's normal range,
 the norm that an optimizer shows, empty lists at the C entry, inference mode, refused gradients, state at odd places,
-lists past the caches.  Tolerances as counted in test_gpu_optimizer."""
+lists past the caches, long lists, layouts under capture, the way to torch's optimizer and back.  Tolerances as counted in
+test_gpu_optimizer."""
 import ctypes
 import math
 
 import pytest
 import torch
 
-from tests.test_gpu_optimizer import (DTYPES, HALF_STEP, NORMS, SIZES, TINY, U, check_clipped, check_step, gen, make,
-                                      make_state, near_norm, norm64, optimizer, params_of, snapshot)
+from tests.test_gpu_optimizer import (B1, B2, DTYPES, EPS, HALF_STEP, LR, NORMS, SIZES, TINY, U, WD, check_clipped, check_step,
+                                      gen, make, make_state, near_norm, norm64, one_step64, optimizer, params_of, snapshot)
 
 pytestmark = pytest.mark.gpu
 
@@ -251,3 +252,100 @@ def test_adamw_of_lists_past_the_caches(dtype):
     check_step(ps, was, states, 11, 0.4 * n / (n + 1e-6))
     for flat, first in zip(flats, (1, 3, 5, 2, 7)):
         ends_kept(flat, total, first)
+
+
+# ---- long lists, scalars, layouts under capture, the other optimizer --------------------------------------------------
+
+@pytest.mark.parametrize('dtype', DTYPES + [DTYPES])
+def test_thousands_of_small_parameters(dtype):
+    """Forty launches of the norm and a hundred of the update; parameters without dimensions among them."""
+    from nerf_amd import ops
+    sizes = [(i * 37) % 71 for i in range(5000)]
+    ps = params_of(sizes, dtype)
+    for i in range(0, 5000, 100):           # (these become scalars)
+        old = ps[i]
+        ps[i] = torch.nn.Parameter(torch.full((), 0.25, device='cuda', dtype=old.dtype))
+        ps[i].grad = torch.full((), -0.01 * (i + 1) / 5000, device='cuda', dtype=old.dtype)
+    states = make_state(ps, 2)
+    was = snapshot(ps, states)
+    grads = [p.grad for p in ps]
+    n = norm64(grads, 2.0)
+    near_norm(ops.grad_norm(grads), n)
+    opt = optimizer(ps, states, max_norm=0.4 * n)
+    opt.step()
+    near_norm(opt.grad_norm, n)
+    check_step(ps, was, states, 3, 0.4 * n / (n + 1e-6))
+    before = [g.double() for g in grads]
+    check_clipped(grads, before, 0.1 * n, 2.0, ops.clip_grad_norm_(grads, 0.1 * n))
+
+
+def test_gradients_of_another_order_in_a_captured_step():
+    """Gradients that are laid out as their parameters inside the captured step, and one that is a broadcast number: each
+    replay reads what they hold then."""
+    from nerf_amd import optim
+
+    def build():
+        a = torch.nn.Parameter(torch.randn(30, 50, device='cuda', generator=gen(1)).t())
+        a.grad = torch.zeros(50, 30, device='cuda')
+        b = torch.nn.Parameter(torch.randn(77, device='cuda', generator=gen(2)))
+        b.grad = torch.zeros(1, device='cuda').expand(77)
+        c = torch.nn.Parameter(torch.randn(64, 3, device='cuda', generator=gen(3)))
+        c.grad = torch.zeros(3, 64, device='cuda').t()
+        return [a, b, c], optim.AdamW([a, b, c], lr=1e-2, max_norm=0.5)
+    ps, opt = build()
+    qs, eager = build()
+    for o in (opt, eager):
+        o.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(4):
+        for p, q in zip(ps, qs):
+            x = torch.randn(p.shape, device='cuda', generator=gen(60 + k))
+            for r in (p, q):
+                if r.grad.stride() == (0,):
+                    r.grad[:1].copy_(x[:1])
+                else:
+                    r.grad.copy_(x)
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(opt.grad_norm, eager.grad_norm)
+        assert all(torch.equal(p.detach(), q.detach()) for p, q in zip(ps, qs))
+
+
+def test_state_to_the_other_optimizer_and_back():
+    """torch's AdamW goes on from a saved state, and this one from torch's: one step from the same state is one step."""
+    from nerf_amd import optim
+    kw = dict(lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD)
+
+    def fill(ps, seed):
+        for p in ps:
+            p.grad = torch.randn(p.shape, device='cuda', generator=gen(seed))
+    ps = params_of(SIZES['network'], torch.float32)
+    mine = optim.AdamW(ps, **kw)
+    for k in range(3):
+        fill(ps, k)
+        mine.step()
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    other = torch.optim.AdamW(qs, fused=True)
+    other.load_state_dict(mine.state_dict())
+    fill(qs, 7)
+    was = [(q.detach().clone(), q.grad.clone(), other.state[q]['exp_avg'].clone(), other.state[q]['exp_avg_sq'].clone()) for q in qs]
+    saved = other.state_dict()
+    back = [torch.nn.Parameter(q.detach().clone()) for q in qs]
+    third = optim.AdamW(back)
+    third.load_state_dict(saved)
+    for p, q in zip(back, qs):
+        p.grad = q.grad.clone()
+    third.step()
+    check_step(back, was, [third.state[p] for p in back], 4, 1.0)
+    other.step()
+    # What torch keeps in fp32 is not ours to say: with beta and its power held in fp32, beta^4 is off by 4 u from beta, 2 u
+    # from the function and u from the difference, so 1 - beta^4 by 7 u / (1 - beta^4): 1750 u for beta2, half of it under
+    # the root, and 20 u for beta1; with the 24 u counted above below 920 u of the ratio.  The weight: three roundings.
+    for q, (w, g, m, v) in zip(qs, was):
+        (want, m1, v1), _ = one_step64(w, g, m, v, 4, 1.0)
+        size = (B1 * m.abs() + (1 - B1) * g.abs()).double() / (1 - B1 ** 4) / ((v1 / (1 - B2 ** 4)).sqrt() + EPS)
+        off = (q.detach().double() - want).abs() - U * (3 * want.abs() + LR * (920 * size + 4 * WD * w.double().abs()))
+        assert bool((off <= 0).all()), float(off.max())
