@@ -66,6 +66,8 @@ class AdamW(torch.optim.Optimizer):
     which a replay reads afresh.  Gradients are taken as they are: where the loss was scaled (fp16), they are divided by the
     scale ahead of the step.  The state is laid out by the first step, which therefore cannot be a captured one."""
 
+    _graph_norm = None      # what grad_norm is from the first captured step on
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, norm_type=2.0,
                  skip_nonfinite=False, *, amsgrad=False, maximize=False, foreach=None, capturable=True, differentiable=False,
                  fused=None):
@@ -83,7 +85,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm = None if max_norm is None else ops.check_max_norm(max_norm)
         self._kind = ops.norm_kind(norm_type)
         self.norm_type, self.skip_nonfinite = float(norm_type), bool(skip_nonfinite)
-        self.grad_norm = self._graph_norm = None
+        self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, capturable=True))
 
     def add_param_group(self, param_group):

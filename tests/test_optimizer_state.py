@@ -126,3 +126,11 @@ def test_a_truth_value_is_no_max_norm(value):
     """The other optimizer's sixth argument is amsgrad: in its place here stands a number."""
     with pytest.raises(ValueError, match='max_norm'):
         optim.AdamW(two(), 1e-3, (0.9, 0.999), 1e-8, 0.01, value)
+
+
+def test_a_copy_made_before_there_was_one_norm_for_all_replays():
+    state = optim.AdamW(two(), max_norm=2.0).__getstate__()
+    assert state.pop('_graph_norm') is None
+    other = optim.AdamW.__new__(optim.AdamW)
+    other.__setstate__(state)
+    assert other._graph_norm is None and other.max_norm == 2.0
