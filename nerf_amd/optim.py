@@ -57,7 +57,8 @@ class AdamW(torch.optim.Optimizer):
 
     `grad_norm` holds the norm of the last step, replays of captured ones included (a 0-d fp32 tensor on the device; None
     before the first step, and without max_norm or skip_nonfinite).  Each step has a tensor of its own until one is captured:
-    from then on it is one tensor, which every later step and every replay write, so that what is to be kept is cloned.
+    from then on it is one tensor, which every later step and every replay write (the first of them: a capture itself runs
+    nothing), so that what is to be kept is cloned.
 
     Parameters are fp32, bf16 or fp16, on one HIP device, their gradients of the same type.  The moments are fp32 whatever
     the parameters are, and a 16-bit parameter has an fp32 master weight in the state ('master'), of which it is the
